@@ -1,0 +1,406 @@
+// Embedding gradient by sorted tokens:
+//   out[v, :] = (accumulate ? out[v, :] : 0) + scale * sum over rows r with tokens[r] == v of dy[r, :]
+// written straight into the 16-bit (or fp32) gradient table, with fp32 sums in a fixed order: equal inputs give equal
+// bits.  Tokens equal to pad_idx or outside [vocab_start, vocab_start + table rows) contribute nothing.
+//
+// What bounds it is memory: every kept row of dy is read once, and either the whole table is written once (new table) or
+// the touched rows are read and written (accumulate).  Three launches:
+//   1. one cluster of eight CTAs sorts (token, row) pairs by a stable radix sort while the other CTAs, when the table is
+//      new, fill it with zeros (the sort hides behind the fill);
+//   2. every warp sums the runs of equal tokens in a piece of `chunk` sorted pairs over 256 columns; runs that lie inside
+//      the piece are final, the first and last run of a piece that cross its border go to fp32 partial rows;
+//   3. runs that cross borders are joined in ascending order.
+// The scatter-add form (embed_ce.cu) needs a zeroed fp32 table, one atomic per element and a pass that folds the table
+// into the 16-bit gradient.
+#include "sm100_common.cuh"
+
+namespace msq {
+
+constexpr int EG_CLUSTER = 8;
+constexpr int EG_SORT_THREADS = 1024;
+constexpr int EG_SORT_WARPS = EG_SORT_THREADS / 32;
+constexpr int EG_MAX_BINS = 512;
+
+__device__ __forceinline__ uint32_t eg_cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void eg_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int eg_ld_remote(const int* p, uint32_t rank) {
+  uint32_t a;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+
+struct EmbedGradSort {
+  const long long* tokens;
+  uint2* buf[2];  // sorted pairs {token - vocab_start or `rows` where nothing is contributed, row}; the result is in buf[passes & 1 ? 0 : 1]
+  int n;
+  long long vocab_start, pad_idx;
+  int rows;      // table rows; the key of pairs that contribute nothing
+  int bits;      // digit width of a pass (at most 9)
+  int passes;
+  uint4* fill;   // table to be zeroed by the other clusters, or null
+  long long fill_vecs;
+};
+
+// Stable least-significant-digit radix sort of n pairs by one cluster of eight CTAs (256 warps, each owning a contiguous
+// part of the input).  Per pass: every warp counts its digits (equal digits of a warp found with match.any, so that
+// ranks inside a warp keep the order), the counts are scanned over warps, CTAs (distributed shared memory) and digits,
+// and every warp writes its pairs to their places.
+__global__ void __cluster_dims__(EG_CLUSTER, 1, 1) __launch_bounds__(EG_SORT_THREADS, 1)
+embed_grad_sort_kernel(const EmbedGradSort s) {
+  extern __shared__ int eg_smem[];
+  int* hist = eg_smem;                              // [warps][bins]
+  int* total = hist + EG_SORT_WARPS * EG_MAX_BINS;  // [bins]: this CTA's counts
+  int* base = total + EG_MAX_BINS;                  // [bins]: first place of this CTA's pairs of a digit
+  int* scan = base + EG_MAX_BINS;                   // [32]
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (blockIdx.x >= EG_CLUSTER) {  // whole clusters: none of their CTAs meets a cluster barrier
+    const long long stride = static_cast<long long>(gridDim.x - EG_CLUSTER) * EG_SORT_THREADS;
+    const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+    for (long long i = static_cast<long long>(blockIdx.x - EG_CLUSTER) * EG_SORT_THREADS + tid; i < s.fill_vecs; i += stride)
+      s.fill[i] = z;
+    return;
+  }
+  const uint32_t rank = eg_cluster_rank();
+  const int bins = 1 << s.bits;
+  const int parts = EG_CLUSTER * EG_SORT_WARPS;
+  const int per = ((s.n + parts - 1) / parts + 31) & ~31;
+  const long long lo = static_cast<long long>(rank * EG_SORT_WARPS + warp) * per;
+  const int first = static_cast<int>(lo < s.n ? lo : s.n);
+  const int last = static_cast<int>(lo + per < s.n ? lo + per : s.n);
+  int* wh = hist + warp * EG_MAX_BINS;
+
+  auto load = [&](int pass, int i) -> uint2 {
+    if (pass == 0) {
+      const long long t = s.tokens[i];
+      const bool in = t != s.pad_idx && t >= s.vocab_start && t < s.vocab_start + s.rows;
+      return make_uint2(in ? static_cast<uint32_t>(t - s.vocab_start) : static_cast<uint32_t>(s.rows), static_cast<uint32_t>(i));
+    }
+    return __ldcg(s.buf[(pass - 1) & 1] + i);
+  };
+
+  for (int pass = 0; pass < s.passes; ++pass) {
+    const int shift = pass * s.bits;
+    for (int b = lane; b < bins; b += 32) wh[b] = 0;
+    __syncwarp();
+    for (int i0 = first; i0 < last; i0 += 32) {
+      const int i = i0 + lane;
+      const bool on = i < last;
+      const uint32_t d = on ? (load(pass, i).x >> shift) & (bins - 1) : 0xFFFFFFFFu;
+      const uint32_t peers = __match_any_sync(0xffffffffu, d);
+      if (on && lane == __ffs(peers) - 1) wh[d] += __popc(peers);
+      __syncwarp();
+    }
+    __syncthreads();
+    for (int b = tid; b < bins; b += EG_SORT_THREADS) {  // exclusive scan over this CTA's warps
+      int run = 0;
+#pragma unroll 8
+      for (int w = 0; w < EG_SORT_WARPS; ++w) {
+        const int t = hist[w * EG_MAX_BINS + b];
+        hist[w * EG_MAX_BINS + b] = run;
+        run += t;
+      }
+      total[b] = run;
+    }
+    __syncthreads();
+    eg_cluster_sync();
+    int before = 0, all = 0;
+    if (tid < bins) {
+#pragma unroll
+      for (uint32_t c = 0; c < EG_CLUSTER; ++c) {
+        const int t = eg_ld_remote(total + tid, c);
+        if (c < rank) before += t;
+        all += t;
+      }
+    }
+    int inc = all;  // inclusive scan over the digits: within warps, then over the warps' sums
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += t;
+    }
+    if (lane == 31) scan[warp] = inc;
+    __syncthreads();
+    if (tid < bins) {
+      int prev = 0;
+      for (int w = 0; w < warp; ++w) prev += scan[w];
+      base[tid] = prev + inc - all + before;
+    }
+    __syncthreads();
+    uint2* dst = s.buf[pass & 1];
+    for (int i0 = first; i0 < last; i0 += 32) {
+      const int i = i0 + lane;
+      const bool on = i < last;
+      const uint2 kv = on ? load(pass, i) : make_uint2(0u, 0u);
+      const uint32_t d = on ? (kv.x >> shift) & (bins - 1) : 0xFFFFFFFFu;
+      const uint32_t peers = __match_any_sync(0xffffffffu, d);
+      int at = 0;
+      if (on) at = base[d] + wh[d] + __popc(peers & ((1u << lane) - 1u));
+      __syncwarp();
+      if (on && lane == __ffs(peers) - 1) wh[d] += __popc(peers);
+      __syncwarp();
+      if (on) __stcg(dst + at, kv);
+    }
+    __threadfence();
+    eg_cluster_sync();  // the pairs are in place, and nobody reads `total` of this pass any more
+  }
+}
+
+template <int DT>  // 0 fp16, 1 bf16, 2 fp32: eight values of a row
+struct Vec8 {
+  uint4 a, b;
+  __device__ __forceinline__ void load(const void* base, long long elem) {
+    if constexpr (DT == 2) {
+      const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(base) + elem);
+      a = __ldcs(p);
+      b = __ldcs(p + 1);
+    } else {
+      a = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + elem));
+    }
+  }
+  __device__ __forceinline__ void add_to(float (&f)[8]) const {
+    if constexpr (DT == 2) {
+      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] += __uint_as_float(w[j]);
+    } else {
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 t = unpack2<DT == 1>(w[j]);
+        f[2 * j] += t.x;
+        f[2 * j + 1] += t.y;
+      }
+    }
+  }
+};
+
+// out[elem .. elem + 7] = (accumulate ? itself : 0) + scale * f, rounded once
+template <int DT>
+__device__ __forceinline__ void store_row8(void* out, long long elem, const float (&f)[8], float scale, int accumulate) {
+  float o[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) o[j] = 0.f;
+  if (accumulate) {
+    Vec8<DT> old;
+    old.load(out, elem);
+    old.add_to(o);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) o[j] = fmaf(f[j], scale, o[j]);
+  if constexpr (DT == 2) {
+    float4* p = reinterpret_cast<float4*>(static_cast<float*>(out) + elem);
+    p[0] = make_float4(o[0], o[1], o[2], o[3]);
+    p[1] = make_float4(o[4], o[5], o[6], o[7]);
+  } else {
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + elem) =
+        make_uint4(pack2<DT == 1>(o[0], o[1]), pack2<DT == 1>(o[2], o[3]), pack2<DT == 1>(o[4], o[5]), pack2<DT == 1>(o[6], o[7]));
+  }
+}
+
+struct EmbedGradSum {
+  const uint2* pairs;
+  const void* dy;
+  long long ldy;
+  void* out;
+  long long ldo;
+  float* head;  // [chunks][D]: sum of a chunk's first run when it began in an earlier chunk
+  float* tail;  // [chunks][D]: sum of a chunk's last run when it begins there and goes on in the next one
+  int n, rows, D, chunk, chunks, slices, accumulate;
+  float scale;
+};
+
+// One warp: `chunk` sorted pairs, 256 columns (eight per lane).  Rows are requested eight at a time so that a warp keeps
+// 4 KB of reads in flight.
+template <int DT>
+__global__ void __launch_bounds__(256) embed_grad_sum_kernel(const EmbedGradSum s) {
+  const long long wid = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  const int c = static_cast<int>(wid / s.slices);
+  if (c >= s.chunks) return;
+  const int col = static_cast<int>(wid - static_cast<long long>(c) * s.slices) * 256 + lane * 8;
+  const bool live = col < s.D;
+  const uint32_t none = static_cast<uint32_t>(s.rows);
+  const int p0 = c * s.chunk, p1 = min(p0 + s.chunk, s.n);
+  const uint32_t prev = p0 > 0 ? s.pairs[p0 - 1].x : none;
+  const uint32_t next = p1 < s.n ? s.pairs[p1].x : none;
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = 0.f;
+  uint32_t run = none;
+  bool first = true;  // no run of this chunk has ended yet
+
+  auto flush = [&](bool at_end) {
+    if (run == none || !live) return;
+    const bool from_before = first && run == prev;
+    const bool goes_on = at_end && run == next;
+    if (from_before || goes_on) {
+      float4* dst = reinterpret_cast<float4*>((from_before ? s.head : s.tail) + static_cast<long long>(c) * s.D + col);
+      dst[0] = make_float4(f[0], f[1], f[2], f[3]);
+      dst[1] = make_float4(f[4], f[5], f[6], f[7]);
+    } else {
+      store_row8<DT>(s.out, static_cast<long long>(run) * s.ldo + col, f, s.scale, s.accumulate);
+    }
+  };
+
+  for (int q0 = p0; q0 < p1; q0 += 32) {
+    const uint2 mine = q0 + lane < p1 ? s.pairs[q0 + lane] : make_uint2(none, 0u);
+    const int cnt = min(32, p1 - q0);
+    for (int e0 = 0; e0 < cnt; e0 += 8) {
+      Vec8<DT> v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t key = __shfl_sync(0xffffffffu, mine.x, e0 + e);
+        const uint32_t row = __shfl_sync(0xffffffffu, mine.y, e0 + e);
+        if (key != none && live) v[e].load(s.dy, static_cast<long long>(row) * s.ldy + col);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t key = __shfl_sync(0xffffffffu, mine.x, e0 + e);
+        if (e0 + e >= cnt) break;
+        if (e0 + e > 0 || q0 > p0) {
+          if (key != run) {
+            flush(false);
+            first = false;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = 0.f;
+          }
+        }
+        run = key;
+        if (key != none && live) v[e].add_to(f);
+      }
+    }
+  }
+  flush(true);
+}
+
+// A run that begins in chunk c and crosses its border: tail[c] + head[c + 1] + ... in ascending order.  A CTA takes 32
+// columns groups of four (128 columns); its eight warps sum contiguous parts of the list, which are then added in order.
+template <int DT>
+__global__ void __launch_bounds__(256) embed_grad_join_kernel(const EmbedGradSum s) {
+  __shared__ float4 part[8][32];
+  const int c = blockIdx.x;
+  const int p1 = (c + 1) * s.chunk;
+  if (p1 >= s.n) return;
+  const uint32_t key = s.pairs[p1 - 1].x;
+  if (key == static_cast<uint32_t>(s.rows) || s.pairs[p1].x != key) return;
+  const int p0 = c * s.chunk;
+  if (p0 > 0 && s.pairs[p0 - 1].x == key) return;  // the run began earlier
+  int lo = p1, hi = s.n;                            // first place behind the run
+  while (lo < hi) {
+    const int mid = lo + ((hi - lo) >> 1);
+    if (s.pairs[mid].x == key) lo = mid + 1; else hi = mid;
+  }
+  const int heads = (lo - 1) / s.chunk - c;  // chunks c + 1 .. c + heads hold the rest
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int col = blockIdx.y * 128 + lane * 4;
+  const bool live = col < s.D;
+  const int per = (heads + 7) >> 3;
+  const int h0 = c + 1 + warp * per, h1 = min(h0 + per, c + 1 + heads);
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (live) {
+    if (warp == 0) a = *reinterpret_cast<const float4*>(s.tail + static_cast<long long>(c) * s.D + col);
+#pragma unroll 8
+    for (int h = h0; h < h1; ++h) {
+      const float4 t = *reinterpret_cast<const float4*>(s.head + static_cast<long long>(h) * s.D + col);
+      a.x += t.x; a.y += t.y; a.z += t.z; a.w += t.w;
+    }
+  }
+  part[warp][lane] = a;
+  __syncthreads();
+  if (warp == 0 && (lane & 1) == 0 && live) {  // eight columns a lane, as everywhere else
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const float4 x = part[w][lane], y = part[w][lane + 1];
+      f[0] += x.x; f[1] += x.y; f[2] += x.z; f[3] += x.w;
+      f[4] += y.x; f[5] += y.y; f[6] += y.z; f[7] += y.w;
+    }
+    store_row8<DT>(s.out, static_cast<long long>(key) * s.ldo + col, f, s.scale, s.accumulate);
+  }
+}
+
+static int eg_chunk(long long n, int D) {
+  const long long slices = (D + 255) / 256;
+  int chunk = 8;
+  while (chunk < 256 && n * slices > 2LL * chunk * 4736) chunk *= 2;
+  return chunk;
+}
+
+}  // namespace msq
+
+// Bytes of scratch (16-byte aligned) that msq_embed_grad_sorted needs for n tokens and D columns.
+extern "C" long long msq_embed_grad_workspace(int n, int D) {
+  const long long chunk = msq::eg_chunk(n, D);
+  const long long chunks = (n + chunk - 1) / chunk;
+  return ((2LL * n * 8 + 255) & ~255LL) + 2LL * chunks * D * 4;
+}
+
+// See the head of this file.  dtype: 0 fp16, 1 bf16, 2 fp32 (dy and out).  D and both row strides are multiples of eight,
+// dy, out and workspace are 16-byte aligned; a new table (accumulate == 0) has contiguous rows (ldo == D).
+extern "C" int msq_embed_grad_sorted(const long long* tokens, const void* dy, long long ldy, void* out, long long ldo, int n,
+                                     int rows, int D, float scale, long long vocab_start, long long pad_idx, int accumulate,
+                                     int dtype, void* workspace, cudaStream_t stream) {
+  using namespace msq;
+  if (n < 0 || n > (1 << 30) || rows <= 0 || D <= 0 || (D & 7) || (ldy & 7) || (ldo & 7) || dtype < 0 || dtype > 2) return -4;
+  if ((reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15) return -4;
+  if (!accumulate && ldo != D) return -4;
+  if (n == 0 && accumulate) return 0;
+  EmbedGradSort so;
+  so.tokens = tokens;
+  so.buf[0] = static_cast<uint2*>(workspace);
+  so.buf[1] = so.buf[0] + n;
+  so.n = n;
+  so.vocab_start = vocab_start;
+  so.pad_idx = pad_idx;
+  so.rows = rows;
+  int bits = 1;
+  while (bits < 31 && (1LL << bits) <= rows) ++bits;  // keys 0 .. rows
+  so.passes = (bits + 8) / 9;
+  so.bits = (bits + so.passes - 1) / so.passes;
+  so.fill = accumulate ? nullptr : static_cast<uint4*>(out);
+  so.fill_vecs = accumulate ? 0 : static_cast<long long>(rows) * D / (dtype == 2 ? 4 : 8);
+  int dev = 0, sms = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const size_t smem = sizeof(int) * (EG_SORT_WARPS * EG_MAX_BINS + 2 * EG_MAX_BINS + 32);
+  if (cudaFuncSetAttribute(embed_grad_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) return -10;
+  const long long fill_ctas = (so.fill_vecs + EG_SORT_THREADS * 4 - 1) / (EG_SORT_THREADS * 4);
+  long long fill_clusters = (fill_ctas + EG_CLUSTER - 1) / EG_CLUSTER;
+  if (fill_clusters > 2 * sms / EG_CLUSTER) fill_clusters = 2 * sms / EG_CLUSTER;
+  embed_grad_sort_kernel<<<static_cast<unsigned>(EG_CLUSTER * (1 + fill_clusters)), EG_SORT_THREADS, smem, stream>>>(so);
+  if (cudaGetLastError() != cudaSuccess) return -11;
+  if (n == 0) return 0;
+  EmbedGradSum su;
+  su.pairs = so.buf[(so.passes - 1) & 1];
+  su.dy = dy; su.ldy = ldy; su.out = out; su.ldo = ldo;
+  su.n = n; su.rows = rows; su.D = D;
+  su.chunk = eg_chunk(n, D);
+  su.chunks = (n + su.chunk - 1) / su.chunk;
+  su.slices = (D + 255) / 256;
+  su.head = reinterpret_cast<float*>(static_cast<char*>(workspace) + ((2LL * n * 8 + 255) & ~255LL));
+  su.tail = su.head + static_cast<long long>(su.chunks) * D;
+  su.accumulate = accumulate; su.scale = scale;
+  const long long warps = static_cast<long long>(su.chunks) * su.slices;
+  const unsigned blocks = static_cast<unsigned>((warps + 7) / 8);
+  const dim3 join(static_cast<unsigned>(su.chunks), static_cast<unsigned>((D + 127) / 128));
+#define MSQ_EG(DT)                                                   \
+  do {                                                               \
+    embed_grad_sum_kernel<DT><<<blocks, 256, 0, stream>>>(su);       \
+    if (su.chunks > 1) embed_grad_join_kernel<DT><<<join, 256, 0, stream>>>(su); \
+  } while (0)
+  if (dtype == 0) MSQ_EG(0);
+  else if (dtype == 1) MSQ_EG(1);
+  else MSQ_EG(2);
+#undef MSQ_EG
+  return cudaGetLastError() == cudaSuccess ? 0 : -11;
+}

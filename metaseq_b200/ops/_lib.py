@@ -27,7 +27,8 @@ F = c_float
 
 # kernels launched by one call of each entry point (used for the launch counter)
 _KERNELS_PER_CALL = {"msq_flash_head_dim_ok": 0, "msq_symm_alloc": 0, "msq_symm_open": 0, "msq_symm_close": 0, "msq_symm_free": 0, "msq_sumsq": 2, "msq_layernorm_bwd": 2, "msq_rmsnorm_bwd": 2, "msq_flash_bwd": 2, "msq_layernorm_bwd_parts": 0,
-                     "msq_sumsq_parts": 0, "msq_gemm2_tiles_n": 0, "msq_gemm_skinny_split": 0, "msq_set_dependent_launch": 0, "msq_gemm_skinny_set_prof": 0, "msq_decode_attn_splits": 0}
+                     "msq_sumsq_parts": 0, "msq_gemm2_tiles_n": 0, "msq_gemm_skinny_split": 0, "msq_set_dependent_launch": 0, "msq_gemm_skinny_set_prof": 0, "msq_decode_attn_splits": 0,
+                     "msq_embed_grad_workspace": 0, "msq_embed_grad_sorted": 3}
 _LAUNCHES = [0]
 
 
@@ -131,6 +132,9 @@ def _declare_kernels(lib):
     for name, sig in _OPTIONAL.items():
         if hasattr(lib, name):
             _sig(lib, name, sig)
+    for name, sig in _SIZES.items():
+        if hasattr(lib, name):
+            _sig(lib, name, sig, L)
 
 
 # Entry points added by later source files; declared when present.
@@ -162,7 +166,12 @@ _OPTIONAL = {
     "msq_gemm2_rowstats": [P, P, P, I, I, I, L, L, L, I, I, I, P, P, P, I, P, P, P],
     "msq_ce_merge_rowstats": [P, P, I, I, P, L, P, I, L, P, P, I, I, I, ctypes.c_uint, I, P],
     "msq_vp_ce_finish_exchanged": [P, L, P, P, I, I, ctypes.c_uint, P, I, I, L, L, F, I, P, P],
+    "msq_embed_grad_sorted": [P, P, L, P, L, I, I, I, F, L, L, I, I, P, P],
     "msq_scale_rows_rel": [P, L, L, I, P, I, I, F, I, P],
+}
+# Workspace queries: bytes (64 bits), no launch.
+_SIZES = {
+    "msq_embed_grad_workspace": [I, I],
 }
 _OPTIONAL = {k: v for k, v in _OPTIONAL.items() if v is not None}
 

@@ -243,18 +243,20 @@ class EmbeddingFn(torch.autograd.Function):
         tokens, positions = ctx.saved_tensors
         tok_w, pos_w = ctx.params
         scale, pad_idx, vstart, nt, np_ = ctx.meta
-        dtok32, dpos32 = F.embed_bwd(tokens, positions, dy.contiguous(), nt, np_, scale, pad_idx, vocab_start=vstart,
-                                     need_pos=pos_w is not None)
+        dy = dy.contiguous()
 
-        def fold(src32, param):
+        def table_grad(index, rows, factor, start, param):
             def compute(out, acc):
-                if out is None:
-                    return src32.to(param.dtype)
-                return F.fold_fp32_into(src32, out, acc)
+                if out is None and param.dtype != dy.dtype:
+                    out = torch.empty((rows, dy.shape[-1]), dtype=param.dtype, device=dy.device)
+                return F.embed_grad_sorted(index, dy, rows, factor, pad_idx, start, out=out, accumulate=acc)
             return _direct_grad(param, compute)
 
-        dt = fold(dtok32, tok_w)
-        dp = fold(dpos32, pos_w) if pos_w is not None else None
+        dt = table_grad(tokens, nt, scale, vstart, tok_w)
+        dp = None
+        if pos_w is not None:  # without position numbers nothing was looked up
+            index = positions if positions is not None else torch.full_like(tokens, pad_idx)
+            dp = table_grad(index, np_, 1.0, 0, pos_w)
         return None, None, dt, dp, None, None, None
 
 

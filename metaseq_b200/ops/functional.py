@@ -632,6 +632,79 @@ def embed_bwd(tokens, positions, dy, tok_rows: int, pos_rows: int, scale: float,
     return dtok, dpos
 
 
+def _float_kernels(t: torch.Tensor) -> bool:
+    """Like ``use_kernels`` for operators whose kernels take 32-bit tensors as well."""
+    if _BACKEND == "torch" or not t.is_cuda or t.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        return False
+    if not _lib.kernels_path().exists():
+        raise RuntimeError("CUDA tensors were passed to metaseq_b200.ops but libmsq_kernels.so is not built; "
+                           "run `python -m metaseq_b200.build_ext`")
+    return True
+
+
+def _same_device(what: str, *tensors):
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"{what}: tensors on different devices ({', '.join(sorted(map(str, devices)))})")
+
+
+def embed_grad_sorted(tokens, dy, rows: int, scale: float = 1.0, pad_idx: int = -1, vocab_start: int = 0,
+                      out: Optional[torch.Tensor] = None, accumulate: bool = False) -> torch.Tensor:
+    """Gradient of an embedding lookup written straight into a table of ``dy``'s type:
+    ``out[v] = (out[v] if accumulate else 0) + scale * sum(dy[r] for tokens[r] - vocab_start == v)``.
+
+    ``tokens``: int64, any shape; ``dy``: ``[*tokens.shape, D]``; ``rows``: rows of the table (this partition's part of
+    the vocabulary).  Tokens equal to ``pad_idx`` or outside the partition contribute nothing; with ``accumulate`` rows
+    that no token names are left as they are.  The sums are formed in fp32 over the rows sorted by token, in a fixed
+    order, and rounded once, so equal inputs give equal bits (``embed_bwd`` adds with atomics, in any order)."""
+    if tokens.dtype != torch.int64:
+        raise ValueError(f"embed_grad_sorted: tokens must be int64, not {tokens.dtype}")
+    if dy.dim() < 1 or dy.shape[:-1] != tokens.shape:
+        raise ValueError(f"embed_grad_sorted: dy {tuple(dy.shape)} does not extend tokens {tuple(tokens.shape)}")
+    D = dy.shape[-1]
+    if rows <= 0 or D <= 0:
+        raise ValueError(f"embed_grad_sorted: the table has no elements (rows={rows}, D={D})")
+    if out is None:
+        if accumulate:
+            raise ValueError("embed_grad_sorted: accumulate needs the table to add to (out)")
+    elif tuple(out.shape) != (rows, D):
+        raise ValueError(f"embed_grad_sorted: out is {tuple(out.shape)}, the table is {(rows, D)}")
+    _same_device("embed_grad_sorted", tokens, dy, out)
+    tok = tokens.reshape(-1).contiguous()
+    dy2 = dy.reshape(-1, D)
+    if dy2.stride(1) != 1 or dy2.stride(0) % 8 or dy2.data_ptr() % 16:
+        dy2 = dy2.contiguous()
+    n = tok.numel()
+    if _float_kernels(dy2) and D % 8 == 0 and dy2.data_ptr() % 16 == 0 and n <= 1 << 30 and (
+            out is None or (out.dtype == dy2.dtype and out.stride(1) == 1 and out.stride(0) % 8 == 0
+                            and (rows == 1 or out.stride(0) >= D) and out.data_ptr() % 16 == 0
+                            and (accumulate or out.is_contiguous()))):
+        lib = _lib.kernels()
+        with torch.cuda.device(dy2.device):
+            if out is None:
+                out = torch.empty((rows, D), dtype=dy2.dtype, device=dy2.device)
+            ws = torch.empty(max(16, lib.msq_embed_grad_workspace(n, D)), dtype=torch.uint8, device=dy2.device)
+            rc = lib.msq_embed_grad_sorted(_lib.ptr(tok), _lib.ptr(dy2), dy2.stride(0), _lib.ptr(out),
+                                           out.stride(0) if rows > 1 else D, n, rows, D, float(scale), int(vocab_start),
+                                           int(pad_idx), int(accumulate), _lib.dtype_code(dy2.dtype), _lib.ptr(ws),
+                                           _lib.stream_ptr())
+        _lib.check_rc(rc, "msq_embed_grad_sorted")
+        return out
+    if dy2.is_cuda and dy2.dtype in (torch.float16, torch.bfloat16) and (out is None or out.dtype == dy2.dtype):
+        _note_fallback("embed_grad_sorted", f"width {D} must be a multiple of 8, the table's rows 16-byte aligned")
+    keep = (tok != pad_idx) & (tok >= vocab_start) & (tok < vocab_start + rows)
+    idx = tok[keep] - vocab_start
+    table = torch.zeros((rows, D), dtype=torch.float32, device=dy2.device)
+    table.index_add_(0, idx, dy2[keep].float() * scale)
+    if out is None:
+        return table.to(dy2.dtype)
+    if not accumulate:
+        return out.copy_(table)
+    hit = torch.unique(idx)
+    out[hit] = (out[hit].float() + table[hit]).to(out.dtype)
+    return out
+
+
 def fold_fp32_into(src32: torch.Tensor, dst16: torch.Tensor, accumulate: bool):
     """``dst16 (+)= src32`` elementwise, with the sum formed in fp32."""
     n = src32.numel()

@@ -1,0 +1,176 @@
+"""Embedding gradient by sorted tokens against its definition in 64 bits, on the CPU and on the GPU.
+
+Bound of an element: the fp32 sum of its k terms and the product with the scale are off by at most
+(k + 2) * 2^-24 * (|old| + scale * sum |dy|), and the one rounding to the table's type by half a step of the result.
+"""
+import pytest
+import torch
+
+from metaseq_b200.ops import autograd as ag
+from metaseq_b200.ops import functional as F
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+DTYPES = [torch.float16, torch.bfloat16, torch.float32]
+
+
+def _oracle(tokens, dy, rows, scale, pad, start, old):
+    """(result, bound of the error before rounding) in 64 bits."""
+    tok = tokens.reshape(-1).cpu()
+    d = dy.reshape(-1, dy.shape[-1]).cpu().double()
+    want = torch.zeros(rows, d.shape[1], dtype=torch.float64) if old is None else old.cpu().double()
+    mass = want.abs()
+    terms = torch.zeros(rows, 1, dtype=torch.float64)
+    keep = (tok != pad) & (tok >= start) & (tok < start + rows)
+    idx = tok[keep] - start
+    want = want.index_add(0, idx, d[keep] * scale)
+    mass = mass.index_add(0, idx, d[keep].abs() * abs(scale))
+    terms = terms.index_add(0, idx, torch.ones(len(idx), 1, dtype=torch.float64))
+    return want, mass * (terms + 2) * 2.0 ** -24
+
+
+def _check(got, want, bound):
+    eps = torch.finfo(got.dtype).eps / 2
+    tiny = torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps / 2  # half a step below the normal range
+    off = (got.cpu().double() - want).abs()
+    assert (off <= bound * 1.01 + eps * (want.abs() + bound) + tiny).all(), float((off - bound - eps * want.abs()).max())
+
+
+def _tokens(kind, n, rows, start, g):
+    if kind == "uniform":
+        return torch.randint(start, start + rows, (n,), generator=g)
+    if kind == "frequent":  # a few tokens make up most of the batch: runs that cross many pieces
+        t = torch.randint(start, start + rows, (n,), generator=g)
+        t[torch.rand(n, generator=g) < 0.8] = start + rows // 2
+        return t
+    if kind == "one":
+        return torch.full((n,), start + rows - 1)
+    if kind == "outside":  # half of them belong to other partitions, on either side
+        return torch.randint(start - rows, start + 2 * rows, (n,), generator=g)
+    if kind == "ascending":
+        return start + torch.arange(n) % rows
+    raise ValueError(kind)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["uniform", "frequent", "one", "outside", "ascending"])
+@pytest.mark.parametrize("n,rows,D", [(1, 1, 8), (7, 3, 8), (33, 130, 264), (257, 511, 520), (1000, 513, 64), (5003, 2050, 136)])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_against_the_definition(device, dtype, kind, n, rows, D, accumulate):
+    g = torch.Generator().manual_seed(n * 31 + D)
+    start, pad = 100, 100 + rows // 3 if rows > 1 else -5
+    tokens = _tokens(kind, n, rows, start, g).to(device)
+    dy = torch.randn(n, D, generator=g).to(dtype).to(device)
+    old = torch.randn(rows, D, generator=g).to(dtype).to(device) if accumulate else None
+    want, bound = _oracle(tokens, dy, rows, 1.5, pad, start, old)
+    out = old.clone() if accumulate else None
+    got = F.embed_grad_sorted(tokens, dy, rows, 1.5, pad, start, out=out, accumulate=accumulate)
+    assert got.dtype == dtype and (out is None or got is out)
+    _check(got, want, bound)
+    if accumulate:
+        named = torch.zeros(rows, dtype=torch.bool)
+        t = tokens.cpu()
+        named[t[(t != pad) & (t >= start) & (t < start + rows)] - start] = True
+        assert torch.equal(got.cpu()[~named], old.cpu()[~named])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_no_tokens_at_all(device):
+    tokens = torch.empty(0, 5, dtype=torch.long, device=device)
+    dy = torch.empty(0, 5, 16, dtype=torch.bfloat16, device=device)
+    assert torch.equal(F.embed_grad_sorted(tokens, dy, 9).float().cpu(), torch.zeros(9, 16))
+    out = torch.ones(9, 16, dtype=torch.bfloat16, device=device)
+    assert (F.embed_grad_sorted(tokens, dy, 9, out=out, accumulate=True) == 1).all()
+    # a batch of padding: nothing is added, and what stands in the padded rows does not matter
+    tokens = torch.full((4,), 3, device=device)
+    dy = torch.full((4, 16), float("nan"), dtype=torch.bfloat16, device=device)
+    assert (F.embed_grad_sorted(tokens, dy, 9, pad_idx=3) == 0).all()
+    assert (F.embed_grad_sorted(tokens, dy, 9, pad_idx=3, out=out, accumulate=True) == 1).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_strided_operands(device):
+    g = torch.Generator().manual_seed(3)
+    tokens = torch.randint(0, 40, (6, 11), generator=g).to(device)
+    wide = torch.randn(6, 11, 48, generator=g).half().to(device)
+    dy = wide[..., 8:40]  # rows 48 apart, 16-byte aligned
+    store = torch.zeros(40, 64, dtype=torch.half, device=device)
+    want, bound = _oracle(tokens, dy, 40, 1.0, -1, 0, store[:, 16:48])
+    _check(F.embed_grad_sorted(tokens, dy, 40, out=store[:, 16:48], accumulate=True), want, bound)
+    assert (store[:, :16] == 0).all() and (store[:, 48:] == 0).all()
+    odd = wide[..., 3:35]  # not aligned
+    want, bound = _oracle(tokens, odd, 40, 1.0, -1, 0, None)
+    _check(F.embed_grad_sorted(tokens, odd, 40), want, bound)
+    broadcast = torch.ones((), dtype=torch.half, device=device).expand(6, 11, 32)  # the gradient of a sum
+    want, bound = _oracle(tokens, broadcast, 40, 1.0, -1, 0, None)
+    _check(F.embed_grad_sorted(tokens, broadcast, 40), want, bound)
+    _check(F.embed_grad_sorted(tokens.t(), broadcast.transpose(0, 1), 40), want, bound)
+
+
+def test_refusals():
+    tokens, dy = torch.zeros(4, dtype=torch.long), torch.zeros(4, 8)
+    with pytest.raises(ValueError, match="int64"):
+        F.embed_grad_sorted(tokens.int(), dy, 3)
+    with pytest.raises(ValueError, match="does not extend"):
+        F.embed_grad_sorted(tokens, dy[:3], 3)
+    with pytest.raises(ValueError, match="accumulate needs"):
+        F.embed_grad_sorted(tokens, dy, 3, accumulate=True)
+    with pytest.raises(ValueError, match="the table is"):
+        F.embed_grad_sorted(tokens, dy, 3, out=torch.zeros(4, 8))
+    with pytest.raises(ValueError, match="no elements"):
+        F.embed_grad_sorted(tokens, dy, 0)
+    with pytest.raises(ValueError, match="different devices"):
+        F.embed_grad_sorted(tokens, dy.to("meta"), 3)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_embedding_backward_uses_it_for_tokens_and_positions(device):
+    torch.manual_seed(0)
+    dt = torch.bfloat16
+    tok_w = torch.randn(50, 24, device=device, dtype=dt).requires_grad_()
+    pos_w = torch.randn(20, 24, device=device, dtype=dt).requires_grad_()
+    tokens = torch.randint(0, 50, (3, 17), device=device)
+    tokens[:, -4:] = 1
+    positions = torch.arange(17, device=device).expand(3, 17) + 2
+    positions = torch.where(tokens == 1, torch.ones_like(positions), positions)
+    y = ag.embedding(tokens, positions, tok_w, pos_w, 2.0, 1)
+    up = torch.randn(y.shape, device=device).to(dt)
+    y.backward(up)
+    want, bound = _oracle(tokens, up, 50, 2.0, 1, 0, None)
+    _check(tok_w.grad, want, bound)
+    want, bound = _oracle(positions, up, 20, 1.0, 1, 0, None)
+    _check(pos_w.grad, want, bound)
+
+
+@pytest.mark.gpu
+def test_equal_inputs_give_equal_bits_and_graph_replay():
+    torch.manual_seed(1)
+    tokens = torch.randint(0, 300, (4096,), device="cuda")
+    tokens[::3] = 7
+    dy = torch.randn(4096, 512, device="cuda", dtype=torch.bfloat16)
+    first = F.embed_grad_sorted(tokens, dy, 300)
+    for _ in range(5):
+        assert torch.equal(F.embed_grad_sorted(tokens, dy, 300), first)
+    out = torch.empty_like(first)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        F.embed_grad_sorted(tokens, dy, 300, out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        F.embed_grad_sorted(tokens, dy, 300, out=out)
+    tokens.copy_(torch.randint(0, 300, (4096,), device="cuda"))
+    out.fill_(float("nan"))
+    graph.replay()
+    assert torch.equal(out, F.embed_grad_sorted(tokens, dy, 300))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,rows,D", [(70001, 50272, 128), (20000, 300000, 8), (3, 1 << 20, 8), (40000, 2, 2048)])
+def test_large_batches_and_tables(n, rows, D):
+    g = torch.Generator(device="cuda").manual_seed(n)
+    tokens = torch.randint(0, rows, (n,), generator=g, device="cuda")
+    dy = torch.randn(n, D, generator=g, device="cuda").half()
+    want, bound = _oracle(tokens, dy, rows, 1.0, -1, 0, None)
+    _check(F.embed_grad_sorted(tokens, dy, rows), want, bound)
