@@ -12,8 +12,11 @@ cuBLAS + unfused-ops baseline the kernels are compared against).
 """
 from __future__ import annotations
 
+import contextlib
+import ctypes
 import logging
 import math
+import operator
 import os
 from typing import Optional
 
@@ -642,6 +645,14 @@ def _float_kernels(t: torch.Tensor) -> bool:
     return True
 
 
+_ANY_DEVICE = contextlib.nullcontext()
+
+
+def _on_device(t: torch.Tensor):
+    """Context in which ``t``'s device is the current one (the kernels launch on the current device's stream)."""
+    return _ANY_DEVICE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
 def _same_device(what: str, *tensors):
     devices = {t.device for t in tensors if t is not None}
     if len(devices) > 1:
@@ -680,7 +691,7 @@ def embed_grad_sorted(tokens, dy, rows: int, scale: float = 1.0, pad_idx: int = 
                             and (rows == 1 or out.stride(0) >= D) and out.data_ptr() % 16 == 0
                             and (accumulate or out.is_contiguous()))):
         lib = _lib.kernels()
-        with torch.cuda.device(dy2.device):
+        with _on_device(dy2):
             if out is None:
                 out = torch.empty((rows, D), dtype=dy2.dtype, device=dy2.device)
             ws = torch.empty(max(16, lib.msq_embed_grad_workspace(n, D)), dtype=torch.uint8, device=dy2.device)
@@ -1145,6 +1156,167 @@ def adamw_step_multi(items, *, lr, beta1, beta2, eps, weight_decay, step, ctrl=N
         float(lr), float(beta1), float(beta2), float(eps), float(weight_decay), float(step_size), _lib.ptr(ctrl),
         _lib.stream_ptr())
     _lib.check_rc(rc, "msq_adamw_multi")
+
+
+# AdamW with 8-bit moments: blocks of ADAMW8_BLOCK consecutive values share one power-of-two scale.
+ADAMW8_BLOCK = 256
+
+
+def adamw8_state(p: torch.Tensor):
+    """Zero moments of ``p`` in the form ``adamw8_step_multi`` takes: ``(m codes, m scales, r codes, r scales)``, the
+    codes ``float8_e4m3fn`` with ``p.numel()`` elements, the scales fp32 with one element per block of 256."""
+    n, blocks = p.numel(), -(-p.numel() // ADAMW8_BLOCK)
+    code = lambda: torch.zeros(n, dtype=torch.uint8, device=p.device).view(torch.float8_e4m3fn)  # noqa: E731
+    scale = lambda: torch.ones(blocks, dtype=torch.float32, device=p.device)  # noqa: E731
+    return code(), scale(), code(), scale()
+
+
+def adamw8_decode(code: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """fp32 values (one dimension) that 8-bit codes and their block scales stand for.  The second moment is held as its
+    root: square the result."""
+    n = code.numel()
+    return code.reshape(-1).float() * scale.repeat_interleave(ADAMW8_BLOCK)[:n]
+
+
+def adamw8_encode(value: torch.Tensor, root: bool = False):
+    """``(codes, scales)`` of fp32 ``value`` rounded to the nearest code; with ``root`` a value above zero is not stored
+    as zero (the rule of the second moment's root).  For states that come from another form."""
+    flat = value.reshape(-1).float()
+    pad = -flat.numel() % ADAMW8_BLOCK
+    blocks = torch.cat([flat, flat.new_zeros(pad)]).view(-1, ADAMW8_BLOCK)
+    half = torch.full(blocks.shape, 0x8000, dtype=torch.int32, device=flat.device)
+    code, scale = _adamw8_round(blocks, half, root)
+    return code.view(-1)[:flat.numel()].contiguous().view(torch.float8_e4m3fn), scale
+
+
+def _adamw8_round(x, rnd, root: bool):
+    """Restatement of the kernel's storage form for ``[blocks, 256]`` fp32 values and 16-bit draws: (uint8, scales)."""
+    mag = x.abs()
+    finite = torch.isfinite(mag)
+    top = torch.where(finite, mag, torch.zeros_like(mag)).amax(dim=1)
+    k = (((top.view(torch.int32) + 0x1FFFFF) >> 23) - (127 + 8)).clamp(-110, 110)
+    scale = ((k + 127) << 23).view(torch.float32)
+    mag = mag * ((127 - k) << 23).view(torch.float32)[:, None]
+    normal = ((mag.view(torch.int32) + (rnd << 4)) >> 20) - (120 << 3)
+    small = torch.where(mag < 0.015625, mag * 512.0 + rnd.float() * (1.0 / 65536.0), torch.zeros_like(mag)).int()
+    code = torch.where(mag < 0.015625, small, normal).clamp(max=0x7E)
+    if root:
+        code = torch.where((code == 0) & (x > 0), torch.ones_like(code), code)
+    code = torch.where(finite, code, torch.full_like(code, 0x7F)) | ((x < 0).int() << 7)
+    return code.to(torch.uint8), scale
+
+
+def _adamw8_draws(blocks: int, first_block: int, seed: int, device):
+    """The two 16-bit draws of every element of a run of blocks: the dropout masks' hash of (seed, element number)."""
+    i = torch.arange(first_block * ADAMW8_BLOCK, (first_block + blocks) * ADAMW8_BLOCK, device=device, dtype=torch.int64)
+
+    def h32(x):
+        x = x ^ (x >> 16)
+        x = (x * 0x7FEB352D) & 0xFFFFFFFF
+        x = x ^ (x >> 15)
+        x = (x * 0x846CA68B) & 0xFFFFFFFF
+        return x ^ (x >> 16)
+
+    bits = h32((i & 0xFFFFFFFF) ^ (seed & 0xFFFFFFFF) ^ h32((i >> 32) ^ ((seed >> 32) & 0xFFFFFFFF)))
+    return (bits & 0xFFFF).int().view(blocks, -1), (bits >> 16).int().view(blocks, -1)
+
+
+_ADAMW8_GRADS = {torch.float16: (torch.float16, torch.float32), torch.bfloat16: (torch.bfloat16, torch.float32),
+                 torch.float32: (torch.float16, torch.bfloat16, torch.float32)}
+_DTYPE_OF, _DEVICE_OF = operator.attrgetter("dtype"), torch.Tensor.get_device  # -1 off the GPU
+
+
+def _adamw8_check(columns):
+    """Refuses lists that the update cannot take.  ``columns``: the parameters, gradients, codes and scales, a tuple
+    each.  Whole lists are looked over at once: a list of a few hundred tensors is common."""
+    p, g, m, ms, r, rs = columns
+    pdt, gdt = set(map(_DTYPE_OF, p)), set(map(_DTYPE_OF, g))
+    if len(pdt) != 1 or len(gdt) != 1 or next(iter(gdt)) not in _ADAMW8_GRADS.get(next(iter(pdt)), ()):
+        raise ValueError("adamw8_step_multi: all parameters share one type, all gradients one type that goes with it "
+                         f"(the parameters' or fp32; any with fp32 parameters), not {pdt} with {gdt}")
+    if set(map(_DTYPE_OF, m)) | set(map(_DTYPE_OF, r)) != {torch.float8_e4m3fn}:
+        raise ValueError("adamw8_step_multi: the codes must be float8_e4m3fn (adamw8_state)")
+    if set(map(_DTYPE_OF, ms)) | set(map(_DTYPE_OF, rs)) != {torch.float32}:
+        raise ValueError("adamw8_step_multi: the scales must be fp32 (adamw8_state)")
+    flat = [t for column in columns for t in column]
+    devices = set(map(_DEVICE_OF, flat))
+    if len(devices) != 1 or (devices == {-1} and len({t.device for t in flat}) != 1):
+        raise ValueError("adamw8_step_multi: tensors on different devices")
+    if not all(map(torch.Tensor.is_contiguous, flat)):
+        raise ValueError("adamw8_step_multi: tensors must be contiguous")
+    numel = torch.Tensor.numel
+    sizes = list(map(numel, p))
+    if not sizes == list(map(numel, g)) == list(map(numel, m)) == list(map(numel, r)):
+        raise ValueError("adamw8_step_multi: a parameter, its gradient and its codes differ in size")
+    if not [-(-n // ADAMW8_BLOCK) for n in sizes] == list(map(numel, ms)) == list(map(numel, rs)):
+        raise ValueError(f"adamw8_step_multi: one scale per block of {ADAMW8_BLOCK} elements is wanted (adamw8_state)")
+    return sizes
+
+
+def adamw8_step_multi(items, *, lr, beta1, beta2, eps, weight_decay, step, seed, ctrl=None):
+    """The AdamW update (decoupled decay, bias correction folded into the step size, eps outside the root) of a list of
+    ``(p, g, m codes, m scales, r codes, r scales)`` whose moments are held in 8 bits (``adamw8_state``); parameters and
+    states are updated in place, in one launch for up to 256 tensors.
+
+    The parameter moves by the moments in fp32.  They are then rounded to one of the two neighbouring codes, up with the
+    probability of the remainder, by a draw from ``seed`` (a non-negative 64-bit number; pass another one every step)
+    and the element's number in the list, so equal calls give equal bits.  Values that are not finite are stored as
+    NaN.  ``ctrl`` is the device control block of ``clip_decision``: gradients are multiplied by ``ctrl[0]`` and nothing
+    changes when ``ctrl[1] != 0``."""
+    items = list(items)
+    if not items:
+        return
+    columns = tuple(zip(*items))
+    if len(columns) != 6:
+        raise ValueError("adamw8_step_multi: items are (p, g, m codes, m scales, r codes, r scales)")
+    sizes = _adamw8_check(columns)
+    if step < 1:
+        raise ValueError(f"adamw8_step_multi: the first step is 1, not {step}")
+    seed = int(seed)
+    if not 0 <= seed < 1 << 64:
+        raise ValueError("adamw8_step_multi: seed must be in [0, 2^64)")
+    p0, g0 = columns[0][0], columns[1][0]
+    if ctrl is not None and (ctrl.dtype != torch.float32 or ctrl.device != p0.device or ctrl.numel() < 2
+                             or not ctrl.is_contiguous()):
+        raise ValueError("adamw8_step_multi: ctrl is the fp32 control block of clip_decision on the tensors' device")
+    step_size = lr * (1.0 - beta2 ** step) ** 0.5 / (1.0 - beta1 ** step)
+    decay, omb1, omb2 = lr * weight_decay, 1.0 - beta1, 1.0 - beta2
+    if _float_kernels(p0):
+        words = [None] * (7 * len(items))
+        for k, column in enumerate(columns):
+            words[k::7] = map(torch.Tensor.data_ptr, column)
+        words[6::7] = sizes
+        with _on_device(p0):
+            rc = _lib.kernels().msq_adamw8_multi((ctypes.c_longlong * len(words))(*words), len(items),
+                                                 _lib.dtype_code(p0.dtype), _lib.dtype_code(g0.dtype), beta1, omb1, beta2,
+                                                 omb2, eps, decay, step_size, seed, _lib.ptr(ctrl), _lib.stream_ptr())
+        _lib.check_rc(rc, "msq_adamw8_multi")
+        return
+    gmul = 1.0
+    if ctrl is not None:
+        if float(ctrl[1]) != 0.0:
+            return
+        gmul = float(ctrl[0])
+    first = 0
+    for (p, g, mc, ms, rc, rs), n in zip(items, sizes):
+        if n == 0:
+            continue
+        nb, pad = ms.numel(), -n % ADAMW8_BLOCK
+        whole = lambda t: torch.cat([t.reshape(-1).float(), t.new_zeros(pad, dtype=torch.float32)]).view(nb, -1)  # noqa: E731
+        g32 = whole(g) * gmul
+        m = whole(mc) * ms[:, None] * beta1 + g32 * omb1
+        r = whole(rc) * rs[:, None]
+        r = torch.sqrt((r * r) * beta2 + (g32 * g32) * omb2)
+        q = whole(p)
+        q = q - q * decay
+        q = q - (m / (r + eps)) * step_size
+        p.copy_(q.view(-1)[:n].view(p.shape))
+        low, high = _adamw8_draws(nb, first, seed, p.device)
+        for code, scale, x, draw, root in ((mc, ms, m, low, False), (rc, rs, r, high, True)):
+            bits, sc = _adamw8_round(x, draw, root)
+            code.view(torch.uint8).view(-1).copy_(bits.view(-1)[:n])
+            scale.copy_(sc)
+        first += nb
 
 
 def adamw_step(p, g, m, v, *, lr, beta1, beta2, eps, weight_decay, step, ctrl=None, p16_out=None):
