@@ -12,7 +12,7 @@
 //   3. runs that cross borders are joined in ascending order.
 // The scatter-add form (embed_ce.cu) needs a zeroed fp32 table, one atomic per element and a pass that folds the table
 // into the 16-bit gradient.
-#include "sm100_common.cuh"
+#include "sm100_pair.cuh"
 
 namespace msq {
 
@@ -21,19 +21,9 @@ constexpr int EG_SORT_THREADS = 1024;
 constexpr int EG_SORT_WARPS = EG_SORT_THREADS / 32;
 constexpr int EG_MAX_BINS = 512;
 
-__device__ __forceinline__ uint32_t eg_cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void eg_cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 __device__ __forceinline__ int eg_ld_remote(const int* p, uint32_t rank) {
-  uint32_t a;
   int v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(map_to_cta(smem_u32(p), rank)) : "memory");
   return v;
 }
 
@@ -68,7 +58,7 @@ embed_grad_sort_kernel(const EmbedGradSort s) {
       s.fill[i] = z;
     return;
   }
-  const uint32_t rank = eg_cluster_rank();
+  const uint32_t rank = cluster_ctarank();
   const int bins = 1 << s.bits;
   const int parts = EG_CLUSTER * EG_SORT_WARPS;
   const int per = ((s.n + parts - 1) / parts + 31) & ~31;
@@ -110,7 +100,7 @@ embed_grad_sort_kernel(const EmbedGradSort s) {
       total[b] = run;
     }
     __syncthreads();
-    eg_cluster_sync();
+    cluster_sync_all();
     int before = 0, all = 0;
     if (tid < bins) {
 #pragma unroll
@@ -149,7 +139,7 @@ embed_grad_sort_kernel(const EmbedGradSort s) {
       if (on) __stcg(dst + at, kv);
     }
     __threadfence();
-    eg_cluster_sync();  // the pairs are in place, and nobody reads `total` of this pass any more
+    cluster_sync_all();  // the pairs are in place, and nobody reads `total` of this pass any more
   }
 }
 

@@ -28,7 +28,8 @@ F = c_float
 # kernels launched by one call of each entry point (used for the launch counter)
 _KERNELS_PER_CALL = {"msq_flash_head_dim_ok": 0, "msq_symm_alloc": 0, "msq_symm_open": 0, "msq_symm_close": 0, "msq_symm_free": 0, "msq_sumsq": 2, "msq_layernorm_bwd": 2, "msq_rmsnorm_bwd": 2, "msq_flash_bwd": 2, "msq_layernorm_bwd_parts": 0,
                      "msq_sumsq_parts": 0, "msq_gemm2_tiles_n": 0, "msq_gemm_skinny_split": 0, "msq_set_dependent_launch": 0, "msq_gemm_skinny_set_prof": 0, "msq_decode_attn_splits": 0,
-                     "msq_embed_grad_workspace": 0, "msq_embed_grad_sorted": 3}
+                     "msq_embed_grad_workspace": 0, "msq_embed_grad_sorted": 3,
+                     "msq_lce_saved_bytes": 0, "msq_lce_fwd_bytes": 0, "msq_lce_bwd_bytes": 0, "msq_lce_fwd": 3, "msq_lce_bwd": 4}
 _LAUNCHES = [0]
 
 
@@ -167,12 +168,17 @@ _OPTIONAL = {
     "msq_ce_merge_rowstats": [P, P, I, I, P, L, P, I, L, P, P, I, I, I, ctypes.c_uint, I, P],
     "msq_vp_ce_finish_exchanged": [P, L, P, P, I, I, ctypes.c_uint, P, I, I, L, L, F, I, P, P],
     "msq_adamw8_multi": [P, I, I, I, F, F, F, F, F, F, F, ctypes.c_ulonglong, P, P],
+    "msq_lce_fwd": [P, L, P, L, P, I, I, I, L, P, P, P, P, I, P, P],
+    "msq_lce_bwd": [P, L, P, I, I, I, L, P, P, P, L, P, L, I, P, I, P, P],
     "msq_embed_grad_sorted": [P, P, L, P, L, I, I, I, F, L, L, I, I, P, P],
     "msq_scale_rows_rel": [P, L, L, I, P, I, I, F, I, P],
 }
 # Workspace queries: bytes (64 bits), no launch.
 _SIZES = {
     "msq_embed_grad_workspace": [I, I],
+    "msq_lce_saved_bytes": [I, I, I],
+    "msq_lce_fwd_bytes": [I, I, I],
+    "msq_lce_bwd_bytes": [I, I, I, I, I],
 }
 _OPTIONAL = {k: v for k, v in _OPTIONAL.items() if v is not None}
 

@@ -230,6 +230,43 @@ def cross_entropy_sum(logits, target, ignore_index: int):
     return CrossEntropyFn.apply(logits, target, ignore_index, getattr(logits, "_msq_row_stats", None))
 
 
+class LinearCrossEntropyFn(torch.autograd.Function):
+    """Summed NLL of ``x @ weight^T`` without the logits (``functional.linear_cross_entropy_fwd``)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, target, ignore_index: int):
+        _, total, saved = F.linear_cross_entropy_fwd(x, weight, target, ignore_index)
+        ctx.save_for_backward(weight, target, *saved)
+        ctx.param = weight
+        ctx.ignore_index = ignore_index
+        return total
+
+    @staticmethod
+    def backward(ctx, g):
+        weight, target, *saved = ctx.saved_tensors
+        need_dx, need_dw = ctx.needs_input_grad[:2]
+        dx = None
+
+        def compute(out, acc):
+            nonlocal dx
+            dx, dw = F.linear_cross_entropy_bwd(saved, weight, target, g, ctx.ignore_index, need_dx, need_dw, dw_out=out,
+                                                accumulate=acc)
+            return dw
+
+        dw = _direct_grad(ctx.param, compute) if need_dw else compute(None, False)
+        return dx, dw, None, None
+
+
+def linear_cross_entropy_sum(x, weight, target, ignore_index: int):
+    """Cross entropy summed over the tokens of ``target`` that are not ``ignore_index``, straight from the features
+    ``x [..., D]`` and the output embedding ``weight [V, D]``: the ``[tokens, V]`` logits are never stored.  Differentiable
+    in ``x`` and ``weight``; the backward pass computes the logits again.  See ``cross_entropy_sum`` for logits that
+    exist already."""
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        return LinearCrossEntropyFn.apply(x, weight, target, ignore_index)
+    return F.linear_cross_entropy_fwd(x, weight, target, ignore_index)[1]
+
+
 class EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, positions, tok_w, pos_w, scale: float, pad_idx: int, vocab_start: int):

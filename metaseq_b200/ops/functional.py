@@ -948,6 +948,141 @@ def scale_rows_(x2d, g, ref: float = 1.0):
     return x2d.mul_(g.to(x2d.dtype).reshape(-1, 1) if g.numel() > 1 else g.to(x2d.dtype))
 
 
+# ------------------------------------------- cross entropy of a linear projection
+_LCE_PIECE = 8192  # vocabulary columns per piece of the PyTorch restatement
+
+
+def _linear_ce_check(x, weight, target):
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"linear_cross_entropy: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not multiply")
+    if target.shape != x.shape[:-1]:
+        raise ValueError(f"linear_cross_entropy: target {tuple(target.shape)} does not go with x {tuple(x.shape)}")
+    if target.dtype != torch.int64:
+        raise ValueError(f"linear_cross_entropy: target must be int64, not {target.dtype}")
+    if x.dtype != weight.dtype or not x.is_floating_point():
+        raise ValueError(f"linear_cross_entropy: x and weight are of one floating type, not {x.dtype} and {weight.dtype}")
+    if weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError("linear_cross_entropy: the weight has no elements")
+    _same_device("linear_cross_entropy", x, weight, target)
+
+
+def _linear_ce_kernel_ok(x2, weight) -> bool:
+    n, D = x2.shape
+    return (use_kernels(x2) and n > 0 and D % 8 == 0 and n <= 1 << 24 and weight.shape[0] <= 1 << 24
+            and weight.stride(1) == 1 and weight.stride(0) % 8 == 0 and weight.stride(0) >= D and weight.data_ptr() % 16 == 0)
+
+
+def linear_cross_entropy_fwd(x, weight, target, ignore_index: int):
+    """Softmax cross entropy of ``x @ weight^T`` without keeping the logits: returns ``(loss, total, saved)``, the loss of
+    every token (fp32, ``target``'s shape, 0 where ``target == ignore_index``), their sum (fp32 scalar) and what
+    ``linear_cross_entropy_bwd`` needs.
+
+    ``x``: ``[..., D]``, ``weight``: ``[V, D]`` of the same type, ``target``: int64.  Rows that are ignored take no part
+    in any product, whatever stands in them.  A target that is neither ``ignore_index`` nor a column of the vocabulary
+    makes the loss of its token NaN.  Logits, sums and statistics are fp32."""
+    _linear_ce_check(x, weight, target)
+    V, D = weight.shape
+    x2, tgt = x.reshape(-1, D), target.reshape(-1).contiguous()
+    n = tgt.numel()
+    ensure_operand_ready(weight)
+    if _linear_ce_kernel_ok(x2, weight):
+        if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.data_ptr() % 16:
+            x2 = x2.contiguous()
+        lib = _lib.kernels()
+        with _on_device(x2):
+            loss = torch.empty(n + 1, dtype=torch.float32, device=x2.device)
+            saved = torch.empty(lib.msq_lce_saved_bytes(n, V, D), dtype=torch.uint8, device=x2.device)
+            ws = torch.empty(lib.msq_lce_fwd_bytes(n, V, D), dtype=torch.uint8, device=x2.device)
+            rc = lib.msq_lce_fwd(_lib.ptr(x2), x2.stride(0), _lib.ptr(weight), weight.stride(0), _lib.ptr(tgt), n, V, D,
+                                 int(ignore_index), _lib.ptr(loss), loss.data_ptr() + 4 * n, _lib.ptr(saved),
+                                 _lib.ptr(ws), _bf(x2), _lib.ptr(_lib.status_word(x2.device)), _lib.stream_ptr())
+        _lib.check_rc(rc, "msq_lce_fwd")
+        return loss[:n].view(target.shape), loss[n], (saved,)
+    if x2.is_cuda and x2.dtype in (torch.float16, torch.bfloat16) and n:
+        _note_fallback("linear_cross_entropy", f"width {D} must be a multiple of 8, weight rows 16-byte aligned")
+    rows = (tgt != ignore_index).nonzero().squeeze(1)
+    xk, tk = x2[rows].float(), tgt[rows]
+    lse = torch.full((len(rows),), float("-inf"), device=x2.device)
+    hit = torch.full((len(rows),), float("nan"), device=x2.device)
+    for v0 in range(0, V, _LCE_PIECE):
+        z = xk @ weight[v0:v0 + _LCE_PIECE].float().t()
+        lse = torch.logaddexp(lse, torch.logsumexp(z, dim=1))
+        here = (tk >= v0) & (tk < v0 + z.shape[1])
+        hit = torch.where(here, z.gather(1, (tk - v0).clamp(0, z.shape[1] - 1)[:, None]).squeeze(1), hit)
+    loss = torch.zeros(n, device=x2.device)
+    loss[rows] = lse - hit
+    return loss.view(target.shape), loss.sum(), (x2, lse)
+
+
+def linear_cross_entropy_bwd(saved, weight, target, g, ignore_index: int, need_dx: bool = True, need_dw: bool = True,
+                             dw_out: Optional[torch.Tensor] = None, accumulate: bool = False):
+    """Gradients ``(dx [*target.shape, D], dw [V, D])`` of ``g * total`` (``g``: one fp32 element on the device).  The
+    logits are computed again, a piece of the vocabulary at a time.  ``dw_out`` receives dw (added to what is there with
+    ``accumulate``: one rounding of the sum)."""
+    V, D = weight.shape
+    tgt = target.reshape(-1).contiguous()
+    n = tgt.numel()
+    if dw_out is not None and tuple(dw_out.shape) != (V, D):
+        raise ValueError(f"linear_cross_entropy_bwd: dw_out is {tuple(dw_out.shape)}, the weight {(V, D)}")
+    if accumulate and dw_out is None:
+        raise ValueError("linear_cross_entropy_bwd: accumulate needs dw_out")
+    _same_device("linear_cross_entropy_bwd", weight, target, g, dw_out)
+    g = g.reshape(1).to(torch.float32)
+    ensure_operand_ready(weight)
+    if len(saved) == 1:
+        lib = _lib.kernels()
+        with _on_device(weight):
+            dx = torch.empty((n, D), dtype=weight.dtype, device=weight.device) if need_dx else None
+            dw = fresh = None
+            if need_dw:
+                direct = dw_out is not None and dw_out.dtype == weight.dtype and dw_out.stride(1) == 1 \
+                    and dw_out.stride(0) % 8 == 0 and dw_out.stride(0) >= D and dw_out.data_ptr() % 16 == 0
+                dw = dw_out if direct else torch.empty((V, D), dtype=weight.dtype, device=weight.device)
+                fresh = None if direct or dw_out is None else dw
+            ws = torch.empty(max(16, lib.msq_lce_bwd_bytes(n, V, D, int(need_dx), int(need_dw))), dtype=torch.uint8,
+                             device=weight.device)
+            rc = lib.msq_lce_bwd(_lib.ptr(weight), weight.stride(0), _lib.ptr(tgt), n, V, D, int(ignore_index),
+                                 _lib.ptr(saved[0]), _lib.ptr(g), _lib.ptr(dx), D, _lib.ptr(dw),
+                                 dw.stride(0) if dw is not None else D, int(accumulate and fresh is None), _lib.ptr(ws),
+                                 _bf(weight), _lib.ptr(_lib.status_word(weight.device)), _lib.stream_ptr())
+        _lib.check_rc(rc, "msq_lce_bwd")
+        if fresh is not None:  # a table of another type or layout
+            dw_out.copy_(dw_out.float() + fresh.float() if accumulate else fresh)
+            dw = dw_out
+        return (dx.view(*target.shape, D) if need_dx else None), dw
+    x2, lse = saved
+    rows = (tgt != ignore_index).nonzero().squeeze(1)
+    xk, tk = x2[rows].float(), tgt[rows]
+    dxk = torch.zeros_like(xk)
+    dw = torch.zeros((V, D), dtype=torch.float32, device=weight.device) if need_dw else None
+    for v0 in range(0, V, _LCE_PIECE):
+        w = weight[v0:v0 + _LCE_PIECE].float()
+        q = torch.exp(xk @ w.t() - lse[:, None])
+        here = ((tk >= v0) & (tk < v0 + len(w))).nonzero().squeeze(1)
+        q[here, tk[here] - v0] -= 1.0
+        if need_dx:
+            dxk += q @ w
+        if need_dw:
+            dw[v0:v0 + len(w)] = q.t() @ xk
+    dx = None
+    if need_dx:
+        dx = torch.zeros((n, D), dtype=weight.dtype, device=weight.device)
+        dx[rows] = (dxk * g).to(weight.dtype)
+        dx = dx.view(*target.shape, D)
+    if need_dw:
+        dw = dw * g
+        if dw_out is not None:
+            dw = dw_out.copy_(dw_out.float() + dw if accumulate else dw)
+        else:
+            dw = dw.to(weight.dtype)
+    return dx, dw
+
+
+def linear_cross_entropy(x, weight, target, ignore_index: int) -> torch.Tensor:
+    """The loss of every token (``linear_cross_entropy_fwd``), without a gradient: validation and scoring."""
+    return linear_cross_entropy_fwd(x, weight, target, ignore_index)[0]
+
+
 # ------------------------------------------------------------------- sampling
 def sample_top_p(lprobs, top_p, uniform=None):
     """One token per row from the nucleus of mass ``top_p`` (a float, or a ``[rows]`` tensor) of fp32
