@@ -192,6 +192,11 @@ def host_path() -> Path:
     return _ROOT / "libmsq_host.so"
 
 
+def kernels_built() -> bool:
+    """True when the CUDA library is there (no look at the file system once it is loaded: operators ask every call)."""
+    return _KLIB is not None or kernels_path().exists()
+
+
 def have_kernels() -> bool:
     """True when the CUDA library is built and a GPU is present to run it."""
     return torch.cuda.is_available() and kernels_path().exists() and not os.environ.get("MSQ_DISABLE_KERNELS")
@@ -224,7 +229,8 @@ def host():
 
 
 def stream_ptr() -> c_void_p:
-    return c_void_p(torch.cuda.current_stream().cuda_stream)
+    """The current stream of the current device (its raw handle: making a ``torch.cuda.Stream`` costs microseconds)."""
+    return c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
 
 
 def ptr(t) -> c_void_p:

@@ -57,7 +57,7 @@ def use_kernels(*tensors) -> bool:
     t = tensors[0]
     if not t.is_cuda or t.dtype not in (torch.float16, torch.bfloat16):
         return False
-    if not _lib.kernels_path().exists():
+    if not _lib.kernels_built():
         raise RuntimeError(
             "CUDA tensors were passed to metaseq_b200.ops but libmsq_kernels.so is not built; "
             "run `python -m metaseq_b200.build_ext`"
@@ -639,7 +639,7 @@ def _float_kernels(t: torch.Tensor) -> bool:
     """Like ``use_kernels`` for operators whose kernels take 32-bit tensors as well."""
     if _BACKEND == "torch" or not t.is_cuda or t.dtype not in (torch.float16, torch.bfloat16, torch.float32):
         return False
-    if not _lib.kernels_path().exists():
+    if not _lib.kernels_built():
         raise RuntimeError("CUDA tensors were passed to metaseq_b200.ops but libmsq_kernels.so is not built; "
                            "run `python -m metaseq_b200.build_ext`")
     return True
@@ -650,12 +650,14 @@ _ANY_DEVICE = contextlib.nullcontext()
 
 def _on_device(t: torch.Tensor):
     """Context in which ``t``'s device is the current one (the kernels launch on the current device's stream)."""
-    return _ANY_DEVICE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _ANY_DEVICE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def _same_device(what: str, *tensors):
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
+    first = tensors[0].device
+    devices = {t.device for t in tensors if t is not None and t.device != first}
+    if devices:
+        devices.add(first)
         raise ValueError(f"{what}: tensors on different devices ({', '.join(sorted(map(str, devices)))})")
 
 
@@ -1092,7 +1094,7 @@ def sample_top_p(lprobs, top_p, uniform=None):
     if uniform is None:
         uniform = torch.rand(rows, device=lprobs.device, dtype=torch.float32)
     per_row = torch.is_tensor(top_p) and top_p.numel() > 1
-    if lprobs.is_cuda and _BACKEND != "torch" and _lib.kernels_path().exists() and lprobs.dtype == torch.float32 \
+    if lprobs.is_cuda and _BACKEND != "torch" and _lib.kernels_built() and lprobs.dtype == torch.float32 \
             and lprobs.stride(1) == 1 and V <= 56000:
         p_t = top_p.to(device=lprobs.device, dtype=torch.float32).contiguous() if torch.is_tensor(top_p) else \
             torch.full((1,), float(top_p), device=lprobs.device, dtype=torch.float32)
@@ -1156,7 +1158,7 @@ def colsum(x2d, out16=None, accumulate=False):
 def sumsq(g: torch.Tensor, out: torch.Tensor, accumulate: bool):
     """``out[0] (+)= sum(g**2)`` in fp32; ``out`` is a 1-element fp32 tensor on ``g``'s device."""
     n = g.numel()
-    if g.is_cuda and _BACKEND != "torch" and g.is_contiguous() and _lib.kernels_path().exists():
+    if g.is_cuda and _BACKEND != "torch" and g.is_contiguous() and _lib.kernels_built():
         lib = _lib.kernels()
         parts = lib.msq_sumsq_parts(n)
         scratch = torch.empty(parts, dtype=torch.float32, device=g.device)
@@ -1206,7 +1208,7 @@ def _tensor_table(tensors):
 
 def list_kernels_ok(tensors) -> bool:
     """True when the list-form kernels take ``tensors``: contiguous CUDA tensors of one 16/32-bit float type."""
-    if not tensors or _BACKEND == "torch" or not tensors[0].is_cuda or not _lib.kernels_path().exists():
+    if not tensors or _BACKEND == "torch" or not tensors[0].is_cuda or not _lib.kernels_built():
         return False
     dt = tensors[0].dtype
     return dt in (torch.float16, torch.bfloat16, torch.float32) and \
@@ -1247,7 +1249,7 @@ def scale_multi_(tensors, dev_scale: Optional[torch.Tensor] = None, host_scale: 
 
 def clip_decision(sumsq_terms: torch.Tensor, pre_factor: float, max_norm: float, ctrl: torch.Tensor):
     """Fills ``ctrl`` (4 fp32): [grad multiplier, skip flag, grad norm, clip coefficient]."""
-    if sumsq_terms.is_cuda and _BACKEND != "torch" and _lib.kernels_path().exists():
+    if sumsq_terms.is_cuda and _BACKEND != "torch" and _lib.kernels_built():
         rc = _lib.kernels().msq_clip_decision(_lib.ptr(sumsq_terms), sumsq_terms.numel(), float(pre_factor),
                                               float(max_norm), _lib.ptr(ctrl), _lib.stream_ptr())
         _lib.check_rc(rc, "msq_clip_decision")
@@ -1329,12 +1331,12 @@ def _adamw8_round(x, rnd, root: bool):
     mag = x.abs()
     finite = torch.isfinite(mag)
     top = torch.where(finite, mag, torch.zeros_like(mag)).amax(dim=1)
-    k = (((top.view(torch.int32) + 0x1FFFFF) >> 23) - (127 + 8)).clamp(-110, 110)
+    k = (((top.view(torch.int32) + 0x1FFFFF) >> 23) - (127 + 8)).clamp(min=-110)
     scale = ((k + 127) << 23).view(torch.float32)
     mag = mag * ((127 - k) << 23).view(torch.float32)[:, None]
     normal = ((mag.view(torch.int32) + (rnd << 4)) >> 20) - (120 << 3)
-    small = torch.where(mag < 0.015625, mag * 512.0 + rnd.float() * (1.0 / 65536.0), torch.zeros_like(mag)).int()
-    code = torch.where(mag < 0.015625, small, normal).clamp(max=0x7E)
+    small = ((torch.where(mag < 0.015625, mag, torch.zeros_like(mag)) * 512.0 + 128.0).view(torch.int32) - 0x43000000 + rnd) >> 16
+    code = torch.where(mag < 0.015625, small, normal)
     if root:
         code = torch.where((code == 0) & (x > 0), torch.ones_like(code), code)
     code = torch.where(finite, code, torch.full_like(code, 0x7F)) | ((x < 0).int() << 7)
@@ -1463,7 +1465,7 @@ def adamw_step(p, g, m, v, *, lr, beta1, beta2, eps, weight_decay, step, ctrl=No
     bc2 = 1.0 - beta2 ** step
     step_size = lr * math.sqrt(bc2) / bc1
     n = p.numel()
-    if p.is_cuda and _BACKEND != "torch" and _lib.kernels_path().exists() and p.is_contiguous() and g.is_contiguous():
+    if p.is_cuda and _BACKEND != "torch" and _lib.kernels_built() and p.is_contiguous() and g.is_contiguous():
         rc = _lib.kernels().msq_adamw(
             _lib.ptr(p), _lib.ptr(g), _lib.ptr(m), _lib.ptr(v), _lib.ptr(p16_out),
             1 if (p16_out is not None and p16_out.dtype == torch.bfloat16) else 0,
