@@ -1335,7 +1335,7 @@ def _adamw8_round(x, rnd, root: bool):
     scale = ((k + 127) << 23).view(torch.float32)
     mag = mag * ((127 - k) << 23).view(torch.float32)[:, None]
     normal = ((mag.view(torch.int32) + (rnd << 4)) >> 20) - (120 << 3)
-    small = ((torch.where(mag < 0.015625, mag, torch.zeros_like(mag)) * 512.0 + 128.0).view(torch.int32) - 0x43000000 + rnd) >> 16
+    small = ((torch.where(mag < 0.015625, mag, torch.zeros_like(mag)) * 2.0 ** 29).round().int() + (rnd << 4)) >> 20
     code = torch.where(mag < 0.015625, small, normal)
     if root:
         code = torch.where((code == 0) & (x > 0), torch.ones_like(code), code)
@@ -1443,7 +1443,8 @@ def adamw8_step_multi(items, *, lr, beta1, beta2, eps, weight_decay, step, seed,
         g32 = whole(g) * gmul
         m = whole(mc) * ms[:, None] * beta1 + g32 * omb1
         r = whole(rc) * rs[:, None]
-        r = torch.sqrt((r * r) * beta2 + (g32 * g32) * omb2)
+        r = (r * r) * beta2 + (g32 * g32) * omb2
+        r = torch.sqrt(torch.where(r < 2.0 ** -126, torch.zeros_like(r), r))  # below fp32's normal range: zero
         q = whole(p)
         q = q - q * decay
         q = q - (m / (r + eps)) * step_size
