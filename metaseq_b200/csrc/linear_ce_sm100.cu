@@ -42,8 +42,9 @@ struct LceParams {
   int M, N, K;
   const int* count;  // kept rows (device memory)
   int count_is;      // 1: the count bounds M, 2: it bounds K
-  int splits;        // the K range is cut into this many parts (LCE_F32)
-  int m_cap;         // rows of one part's slab of the fp32 output
+  int pairs;         // CTA pairs of a full grid (LCE_F32: lce_splits)
+  int split_k;       // K blocks that the number of parts is chosen for
+  int slab_rows;     // rows of the fp32 output; a part has a slab of M rows rounded up to 256
   int accumulate;
   int bf16;
   int* status;
@@ -86,6 +87,24 @@ __device__ __forceinline__ void lce_tile_coords(int tile, int tiles_m, int tiles
   tn = r / gsize;
 }
 
+// Parts into which K is cut so that few tiles fill the machine: the number that makes the waves shortest, in units of a
+// fifth of one k block of a tile (0.4 us); thirty for the start and end of a wave, one per tile for a further slab's way to
+// memory and back.  The kernels find the same number from the rows that are really there.
+__host__ __device__ inline int lce_splits(int tiles, int k_blocks, int most, int pairs) {
+  int best = 1;
+  long long best_cost = 0;
+  if (most > 32) most = 32;
+  for (int s = 1; s <= most && (s == 1 || s * 4 <= k_blocks); ++s) {
+    const long long waves = (tiles * s + pairs - 1) / pairs;
+    const long long cost = 5 * waves * ((k_blocks + s - 1) / s + 6) + static_cast<long long>(tiles) * (s - 1);
+    if (s == 1 || cost < best_cost) {
+      best_cost = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+
 template <bool A_MN, bool B_MN, int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LC_THREADS, 1)
 lce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -115,9 +134,11 @@ lce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   const int tiles_m = (M + 2 * LC_BM - 1) / (2 * LC_BM);
   const int tiles_n = (p.N + LC_BN - 1) / LC_BN;
   const int tiles = tiles_m * tiles_n;
-  const int num_items = tiles * p.splits;
+  const int m_cap = tiles_m * 2 * LC_BM;
+  const int splits = EPI == LCE_F32 && tiles > 0 ? lce_splits(tiles, p.count_is == 2 ? (K + LC_BK - 1) / LC_BK : p.split_k, p.slab_rows / m_cap, p.pairs) : 1;
+  const int num_items = tiles * splits;
   const int k_total = (K + LC_BK - 1) / LC_BK;
-  const int k_per = (k_total + p.splits - 1) / p.splits;
+  const int k_per = (k_total + splits - 1) / splits;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < LC_STAGES; ++s) {
@@ -347,7 +368,7 @@ lce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           const int col0 = col_base + c * 32;
-          if (col0 >= p.N || row_base >= M) break;
+          if (col0 >= p.N || row_base >= M || (empty && p.accumulate)) break;
           uint32_t r[32];
           tmem_ld_32x32(taddr + c * 32, r);
           tmem_ld_wait();
@@ -360,8 +381,8 @@ lce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            if (p.accumulate) tma_reduce_add_2d(&tmC, stage, col0, split * p.m_cap + row_base);
-            else tma_store_2d(&tmC, stage, col0, split * p.m_cap + row_base);
+            if (p.accumulate) tma_reduce_add_2d(&tmC, stage, col0, split * m_cap + row_base);
+            else tma_store_2d(&tmC, stage, col0, split * m_cap + row_base);
             bulk_commit_group();
           }
         }
@@ -569,7 +590,9 @@ __global__ void __launch_bounds__(256) lce_merge_kernel(const LceMerge s) {
 // Rows of `out` that no kept row names are cleared by the second half of the grid's y range (zero_target).
 struct LceFinish {
   const float* acc;
-  int parts, m_cap, D, M;
+  int pairs, split_k, slab_rows;  // as for the product that left the parts
+  const int* split_count;         // its K is the count (rows null), or null
+  int D, M;
   const int* rows;
   const int* count;           // bounds the rows, or null
   const long long* target;    // with rows: [M] targets by original row
@@ -585,7 +608,10 @@ __global__ void __launch_bounds__(256) lce_finish_kernel(const LceFinish s) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int M = s.count ? *s.count : s.M;
   const float alpha = s.g ? s.alpha * *s.g : s.alpha;
-  const long long slab = static_cast<long long>(s.m_cap) * s.D;
+  const int m_cap = (M + 2 * LC_BM - 1) / (2 * LC_BM) * (2 * LC_BM);
+  const int tiles = m_cap / (2 * LC_BM) * ((s.D + LC_BN - 1) / LC_BN);
+  const int parts = tiles > 0 ? lce_splits(tiles, s.split_count ? (*s.split_count + LC_BK - 1) / LC_BK : s.split_k, s.slab_rows / m_cap, s.pairs) : 1;
+  const long long slab = static_cast<long long>(m_cap) * s.D;
   for (int r = blockIdx.x * 8 + warp; r < s.M; r += gridDim.x * 8) {
     if (s.rows && s.target[r] == s.ignore) {
       uint16_t* o = s.out + static_cast<long long>(r) * s.ldo;
@@ -599,7 +625,7 @@ __global__ void __launch_bounds__(256) lce_finish_kernel(const LceFinish s) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] = 0.f;
 #pragma unroll 4
-      for (int q = 0; q < s.parts; ++q) {
+      for (int q = 0; q < parts; ++q) {
         const float4 x = *reinterpret_cast<const float4*>(a + q * slab + c), y = *reinterpret_cast<const float4*>(a + q * slab + c + 4);
         f[0] += x.x; f[1] += x.y; f[2] += x.z; f[3] += x.w;
         f[4] += y.x; f[5] += y.y; f[6] += y.z; f[7] += y.w;
@@ -636,7 +662,7 @@ static int lce_launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUte
                       cudaStream_t stream) {
   auto kern = lce_gemm_kernel<A_MN, B_MN, EPI>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, LC_SMEM) != cudaSuccess) return -10;
-  const long long items = static_cast<long long>((p.M + 2 * LC_BM - 1) / (2 * LC_BM)) * ((p.N + LC_BN - 1) / LC_BN) * p.splits;
+  const long long items = static_cast<long long>((p.M + 2 * LC_BM - 1) / (2 * LC_BM)) * ((p.N + LC_BN - 1) / LC_BN) * (EPI == LCE_F32 ? 32 : 1);
   long long pairs = sms / 2;
   if (pairs > items) pairs = items;
   if (pairs <= 0) return 0;
@@ -660,30 +686,48 @@ static long long lce_align(long long b) { return (b + 255) & ~255LL; }
 
 // How the backward pass is cut up.
 struct LcePlan {
-  int piece;      // columns of the vocabulary per piece
-  int dx_splits;  // parts of the piece (K) in dx += P w
-  int dw_splits;  // parts of the rows (K) in dw = P^T x; 1: written directly
+  int piece;           // columns of the vocabulary per piece
+  long long dx_rows;   // rows of dx's fp32 slabs
+  long long dw_rows;   // rows of dw's fp32 slabs; 0: one part, written directly
 };
 
+// The size of a piece is the one whose three products have the shortest waves (units as in lce_splits, ten for a launch),
+// P staying within 256 MB; ignored rows are not known here.  16384 rows, 50272 columns, width 2048: pieces of 4096 columns
+// (dw: 128 tiles for 74 pairs) 11.34 ms, of 4608 (144 tiles) 11.11 ms.
 static LcePlan lce_plan(int n, int V, int D, int sms) {
   LcePlan q;
   const int pairs = sms / 2;
-  const long long tn_d = (D + LC_BN - 1) / LC_BN;
-  const long long tm_n = (n + 2 * LC_BM - 1) / (2 * LC_BM);
-  // a piece of P of about 128 MB
-  long long piece = (128LL << 20) / (2LL * n) / 256 * 256;
-  if (piece < 1024) piece = 1024;
-  const long long vcap = (static_cast<long long>(V) + 255) / 256 * 256;
-  if (piece > vcap) piece = vcap;
-  q.piece = static_cast<int>(piece);
-  long long s = pairs / (tm_n * tn_d);
-  long long most = (piece + LC_BK - 1) / LC_BK / 4;  // at least four k blocks a part
-  if (s > most) s = most;
-  q.dx_splits = static_cast<int>(s < 1 ? 1 : s);
-  s = pairs / (((piece + 2 * LC_BM - 1) / (2 * LC_BM)) * tn_d);
-  most = (static_cast<long long>(n) + LC_BK - 1) / LC_BK / 4;
-  if (s > most) s = most;
-  q.dw_splits = static_cast<int>(s < 1 ? 1 : s);
+  const int tn_d = (D + LC_BN - 1) / LC_BN, tm_n = (n + 2 * LC_BM - 1) / (2 * LC_BM), tv = (V + 255) / 256;
+  const int k_d = (D + LC_BK - 1) / LC_BK, k_n = (n + LC_BK - 1) / LC_BK;
+  long long most = (256LL << 20) / (512LL * n);
+  if (most > tv) most = tv;
+  if (most < 4) most = tv < 4 ? tv : 4;
+  auto waves = [&](long long tiles) { return (tiles + pairs - 1) / pairs; };
+  auto cost = [&](long long t) -> double {  // of a piece of t tiles
+    const int s = lce_splits(static_cast<int>(tm_n * tn_d), static_cast<int>(t * 4), 32, pairs);
+    const int u = lce_splits(static_cast<int>(t * tn_d), k_n, 32, pairs);
+    return 30.0 + waves(tm_n * t) * (k_d + 6) + waves(static_cast<long long>(tm_n) * tn_d * s) * ((t * 4 + s - 1) / s + 6) +
+           waves(t * tn_d * u) * ((k_n + u - 1) / u + 6);
+  };
+  long long piece = most;
+  double best = 1e300;
+  auto consider = [&](long long t) {
+    if (t < 1 || t > most) return;
+    const long long whole = tv / t, rest = tv - whole * t;
+    const double c = whole * cost(t) + (rest ? cost(rest) : 0.0);
+    if (c < best) {
+      best = c;
+      piece = t;
+    }
+  };
+  const long long fewest = (tv + most - 1) / most;
+  for (long long k = fewest; k <= fewest + 6; ++k) consider((tv + k - 1) / k);      // pieces of equal size
+  for (long long w = 1; w <= 8; ++w) consider(w * pairs / tn_d);                      // whole waves of dw's tiles
+  q.piece = static_cast<int>(piece * 256);
+  const int s = lce_splits(tm_n * tn_d, static_cast<int>(piece * 4), 32, pairs);
+  const int u = lce_splits(static_cast<int>(piece) * tn_d, k_n, 32, pairs);
+  q.dx_rows = static_cast<long long>(s) * tm_n * 256;
+  q.dw_rows = u > 1 ? u * piece * 256 : 0;
   return q;
 }
 
@@ -736,10 +780,9 @@ extern "C" long long msq_lce_bwd_bytes(int n, int V, int D, int need_dx, int nee
   using namespace msq;
   if (!lce_sizes_ok(n, V, D)) return -1;
   const LcePlan q = lce_plan(n, V, D, lce_sms());
-  const long long n_cap = (n + 255) / 256 * 256LL, v_cap = (q.piece + 255) / 256 * 256LL;
   long long b = lce_align(2LL * n * q.piece);
-  if (need_dx) b += lce_align(4LL * q.dx_splits * n_cap * D);
-  if (need_dw && q.dw_splits > 1) b += lce_align(4LL * q.dw_splits * v_cap * D);
+  if (need_dx) b += lce_align(4LL * q.dx_rows * D);
+  if (need_dw) b += lce_align(4LL * q.dw_rows * D);
   return b;
 }
 
@@ -776,7 +819,7 @@ extern "C" int msq_lce_fwd(const void* x, long long ldx, const void* w, long lon
   if (rc) return rc;
   LceParams p = {};
   p.M = n; p.N = V; p.K = D;
-  p.count = sv.count; p.count_is = 1; p.splits = 1;
+  p.count = sv.count; p.count_is = 1;
   p.bf16 = bf16; p.status = status;
   p.target = sv.tgt;
   p.st_max = st_max; p.st_sum = st_sum; p.st_tgt = st_tgt;
@@ -802,12 +845,11 @@ extern "C" int msq_lce_bwd(const void* w, long long ldw, const long long* target
   const int sms = lce_sms();
   const LceSaved sv = lce_saved(const_cast<void*>(saved), n, D);
   const LcePlan q = lce_plan(n, V, D, sms);
-  const int n_cap = (n + 255) / 256 * 256, v_cap = (q.piece + 255) / 256 * 256;
   char* at = static_cast<char*>(ws);
   uint16_t* P = reinterpret_cast<uint16_t*>(at);
   at += lce_align(2LL * n * q.piece);
   float* dx32 = reinterpret_cast<float*>(at);
-  if (dx) at += lce_align(4LL * q.dx_splits * n_cap * D);
+  if (dx) at += lce_align(4LL * q.dx_rows * D);
   float* dw32 = reinterpret_cast<float*>(at);
   // fp16 cannot hold the probabilities of a large vocabulary as they are (2e-5 is below its normal range): P is stored
   // times 2^15 and the factor taken out of the fp32 sums.  |P| <= 1.
@@ -823,7 +865,7 @@ extern "C" int msq_lce_bwd(const void* w, long long ldw, const long long* target
     const uint16_t* wp = static_cast<const uint16_t*>(w) + static_cast<long long>(v0) * ldw;
     CUtensorMap tmW, tmWmn, tmP, tmPk, tmPmn, tmOut;
     LceParams p = {};
-    p.count = sv.count; p.bf16 = bf16; p.status = status; p.splits = 1; p.alpha = alpha;
+    p.count = sv.count; p.bf16 = bf16; p.status = status; p.alpha = alpha; p.pairs = sms / 2;
     // P = (softmax - onehot) of this piece
     if ((rc = make_tmap_2d(&tmW, wp, pv, D, ldw, LC_BN / 2, bf16))) return rc;
     if ((rc = lce_out_map(&tmP, P, n, pv, q.piece, false, bf16))) return rc;
@@ -833,20 +875,20 @@ extern "C" int msq_lce_bwd(const void* w, long long ldw, const long long* target
     if (dx) {
       if ((rc = make_tmap_2d(&tmPk, P, n, pv, q.piece, LC_BM, bf16))) return rc;
       if ((rc = make_tmap_2d(&tmWmn, wp, pv, D, ldw, LC_BK, bf16))) return rc;
-      if ((rc = lce_out_map(&tmOut, dx32, static_cast<long long>(q.dx_splits) * n_cap, D, D, true, bf16))) return rc;
-      p.M = n; p.N = D; p.K = pv; p.count_is = 1; p.splits = q.dx_splits; p.m_cap = n_cap; p.accumulate = v0 > 0;
+      if ((rc = lce_out_map(&tmOut, dx32, q.dx_rows, D, D, true, bf16))) return rc;
+      p.M = n; p.N = D; p.K = pv; p.count_is = 1; p.split_k = q.piece / LC_BK; p.slab_rows = static_cast<int>(q.dx_rows); p.accumulate = v0 > 0;
       if ((rc = lce_launch<false, true, LCE_F32>(tmPk, tmWmn, tmOut, p, sms, stream))) return rc;
     }
     if (dw) {
       uint16_t* dwp = static_cast<uint16_t*>(dw) + static_cast<long long>(v0) * lddw;
       if ((rc = make_tmap_2d(&tmPmn, P, n, pv, q.piece, LC_BK, bf16))) return rc;
-      p.M = pv; p.N = D; p.K = n; p.count_is = 2; p.splits = q.dw_splits; p.m_cap = v_cap;
-      if (q.dw_splits > 1) {
-        if ((rc = lce_out_map(&tmOut, dw32, static_cast<long long>(q.dw_splits) * v_cap, D, D, true, bf16))) return rc;
+      p.M = pv; p.N = D; p.K = n; p.count_is = 2; p.slab_rows = static_cast<int>(q.dw_rows);
+      if (q.dw_rows > 0) {
+        if ((rc = lce_out_map(&tmOut, dw32, q.dw_rows, D, D, true, bf16))) return rc;
         p.accumulate = 0;
         if ((rc = lce_launch<true, true, LCE_F32>(tmPmn, tmXmn, tmOut, p, sms, stream))) return rc;
         LceFinish f = {};
-        f.acc = dw32; f.parts = q.dw_splits; f.m_cap = v_cap; f.D = D; f.M = pv;
+        f.acc = dw32; f.pairs = sms / 2; f.slab_rows = p.slab_rows; f.split_count = sv.count; f.D = D; f.M = pv;
         f.out = dwp; f.ldo = lddw; f.g = g; f.alpha = alpha; f.accumulate = accumulate; f.bf16 = bf16;
         const int blocks = (pv + 7) / 8;
         lce_finish_kernel<<<blocks < 8 * sms ? blocks : 8 * sms, 256, 0, stream>>>(f);
@@ -859,7 +901,7 @@ extern "C" int msq_lce_bwd(const void* w, long long ldw, const long long* target
   }
   if (dx) {
     LceFinish f = {};
-    f.acc = dx32; f.parts = q.dx_splits; f.m_cap = n_cap; f.D = D; f.M = n;
+    f.acc = dx32; f.pairs = sms / 2; f.split_k = q.piece / LC_BK; f.slab_rows = static_cast<int>(q.dx_rows); f.D = D; f.M = n;
     f.rows = sv.rows; f.count = sv.count; f.target = target; f.ignore = ignore;
     f.out = static_cast<uint16_t*>(dx); f.ldo = lddx; f.g = g; f.alpha = alpha; f.bf16 = bf16;
     const int blocks = (n + 7) / 8;
