@@ -4,12 +4,15 @@
 // bits.  Tokens equal to pad_idx or outside [vocab_start, vocab_start + table rows) contribute nothing.
 //
 // What bounds it is memory: every kept row of dy is read once, and either the whole table is written once (new table) or
-// the touched rows are read and written (accumulate).  Three launches:
+// the touched rows are read and written (accumulate).  Up to 1024 tokens one kernel does everything (after a zero fill of a
+// new table): every CTA sorts all tokens in shared memory and sums 256 columns.  Above that, three launches:
 //   1. one cluster of eight CTAs sorts (token, row) pairs by a stable radix sort while the other CTAs, when the table is
-//      new, fill it with zeros (the sort hides behind the fill);
+//      new, fill its first rows with zeros;
 //   2. every warp sums the runs of equal tokens in a piece of `chunk` sorted pairs over 256 columns; runs that lie inside
-//      the piece are final, the first and last run of a piece that cross its border go to fp32 partial rows;
+//      the piece are final, the first and last run of a piece that cross its border go to fp32 partial rows.  Further
+//      CTAs clear the rest of a new table, leaving out the rows that a token names (found in the sorted pairs);
 //   3. runs that cross borders are joined in ascending order.
+// The launches are chained (programmatic dependent launch), each starts while its predecessor drains.
 // The scatter-add form (embed_ce.cu) needs a zeroed fp32 table, one atomic per element and a pass that folds the table
 // into the 16-bit gradient.
 #include "sm100_pair.cuh"
@@ -51,6 +54,7 @@ embed_grad_sort_kernel(const EmbedGradSort s) {
   int* base = total + EG_MAX_BINS;                  // [bins]: first place of this CTA's pairs of a digit
   int* scan = base + EG_MAX_BINS;                   // [32]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  dependents_launch();
   if (blockIdx.x >= EG_CLUSTER) {  // whole clusters: none of their CTAs meets a cluster barrier
     const long long stride = static_cast<long long>(gridDim.x - EG_CLUSTER) * EG_SORT_THREADS;
     const uint4 z = make_uint4(0u, 0u, 0u, 0u);
@@ -205,13 +209,48 @@ struct EmbedGradSum {
   float* tail;  // [chunks][D]: sum of a chunk's last run when it begins there and goes on in the next one
   int n, rows, D, chunk, chunks, slices, accumulate;
   float scale;
+  int fill_blocks;  // the first CTAs clear rows fill_from .. rows - 1 of a new table, the others sum
+  int fill_from;
 };
+
+// Rows of a new table that no token names, 32 rows a warp at a time: every lane looks its row up in the sorted pairs.
+template <int DT>
+__device__ void embed_grad_fill(const EmbedGradSum& s) {
+  constexpr int PER = DT == 2 ? 4 : 8;  // elements of 16 bytes
+  const int lane = threadIdx.x & 31, vecs = s.D / PER;
+  const int warps = s.fill_blocks * 8;
+  const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+  for (long long r0 = s.fill_from + 32LL * (blockIdx.x * 8 + (threadIdx.x >> 5)); r0 < s.rows; r0 += 32LL * warps) {
+    const long long row = r0 + lane;
+    bool clear = row < s.rows;
+    if (clear) {
+      int lo = 0, hi = s.n;  // first pair whose token is not below the row
+      while (lo < hi) {
+        const int mid = lo + ((hi - lo) >> 1);
+        if (s.pairs[mid].x < static_cast<uint32_t>(row)) lo = mid + 1; else hi = mid;
+      }
+      clear = lo == s.n || s.pairs[lo].x != static_cast<uint32_t>(row);
+    }
+    const unsigned mask = __ballot_sync(0xffffffffu, clear);
+    for (int k = 0; k < 32; ++k) {
+      if (!((mask >> k) & 1u)) continue;
+      uint4* dst = static_cast<uint4*>(s.out) + (r0 + k) * vecs;
+      for (int v = lane; v < vecs; v += 32) dst[v] = z;
+    }
+  }
+}
 
 // One warp: `chunk` sorted pairs, 256 columns (eight per lane).  Rows are requested eight at a time so that a warp keeps
 // 4 KB of reads in flight.
 template <int DT>
 __global__ void __launch_bounds__(256) embed_grad_sum_kernel(const EmbedGradSum s) {
-  const long long wid = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  dependents_launch();
+  dependents_wait();
+  if (static_cast<int>(blockIdx.x) < s.fill_blocks) {
+    embed_grad_fill<DT>(s);
+    return;
+  }
+  const long long wid = static_cast<long long>(blockIdx.x - s.fill_blocks) * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   const int c = static_cast<int>(wid / s.slices);
   if (c >= s.chunks) return;
@@ -271,52 +310,232 @@ __global__ void __launch_bounds__(256) embed_grad_sum_kernel(const EmbedGradSum 
   flush(true);
 }
 
-// A run that begins in chunk c and crosses its border: tail[c] + head[c + 1] + ... in ascending order.  A CTA takes 32
-// columns groups of four (128 columns); its eight warps sum contiguous parts of the list, which are then added in order.
+// Runs that begin in chunk c and cross its border: tail[c] + head[c + 1] + ... in ascending order, 256 columns per warp.  A
+// CTA looks after EG_JOIN chunks (most have nothing to join); runs over more than EG_LONG chunks are summed by all its
+// warps, each a contiguous part, and the parts added in order.
+constexpr int EG_JOIN = 16;
+constexpr int EG_LONG = 64;
+
 template <int DT>
 __global__ void __launch_bounds__(256) embed_grad_join_kernel(const EmbedGradSum s) {
-  __shared__ float4 part[8][32];
-  const int c = blockIdx.x;
-  const int p1 = (c + 1) * s.chunk;
-  if (p1 >= s.n) return;
-  const uint32_t key = s.pairs[p1 - 1].x;
-  if (key == static_cast<uint32_t>(s.rows) || s.pairs[p1].x != key) return;
-  const int p0 = c * s.chunk;
-  if (p0 > 0 && s.pairs[p0 - 1].x == key) return;  // the run began earlier
-  int lo = p1, hi = s.n;                            // first place behind the run
-  while (lo < hi) {
-    const int mid = lo + ((hi - lo) >> 1);
-    if (s.pairs[mid].x == key) lo = mid + 1; else hi = mid;
-  }
-  const int heads = (lo - 1) / s.chunk - c;  // chunks c + 1 .. c + heads hold the rest
+  __shared__ float part[8][8][32];
+  __shared__ int long_runs[EG_JOIN][2];
+  __shared__ int long_count;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int col = blockIdx.y * 128 + lane * 4;
+  const int col = blockIdx.y * 256 + lane * 8;
   const bool live = col < s.D;
-  const int per = (heads + 7) >> 3;
-  const int h0 = c + 1 + warp * per, h1 = min(h0 + per, c + 1 + heads);
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (live) {
-    if (warp == 0) a = *reinterpret_cast<const float4*>(s.tail + static_cast<long long>(c) * s.D + col);
-#pragma unroll 8
-    for (int h = h0; h < h1; ++h) {
-      const float4 t = *reinterpret_cast<const float4*>(s.head + static_cast<long long>(h) * s.D + col);
-      a.x += t.x; a.y += t.y; a.z += t.z; a.w += t.w;
-    }
-  }
-  part[warp][lane] = a;
+  const uint32_t none = static_cast<uint32_t>(s.rows);
+  if (threadIdx.x == 0) long_count = 0;
   __syncthreads();
-  if (warp == 0 && (lane & 1) == 0 && live) {  // eight columns a lane, as everywhere else
+  dependents_wait();
+
+  auto add = [&](const float* from, int chunk, float (&f)[8]) {
+    const float4* q = reinterpret_cast<const float4*>(from + static_cast<long long>(chunk) * s.D + col);
+    const float4 x = q[0], y = q[1];
+    f[0] += x.x; f[1] += x.y; f[2] += x.z; f[3] += x.w;
+    f[4] += y.x; f[5] += y.y; f[6] += y.z; f[7] += y.w;
+  };
+
+  for (int c = blockIdx.x * EG_JOIN + warp; c < min((static_cast<int>(blockIdx.x) + 1) * EG_JOIN, s.chunks - 1); c += 8) {
+    const int p0 = c * s.chunk, p1 = p0 + s.chunk;
+    const uint32_t before = p0 > 0 ? s.pairs[p0 - 1].x : none, key = s.pairs[p1 - 1].x, after = s.pairs[p1].x;
+    if (key == none || after != key || before == key) continue;  // nothing crosses, or it began earlier
+    int heads = 0;  // chunks behind c that begin with this token
+    while (true) {
+      const int q = c + 1 + heads + lane;
+      const unsigned same = __ballot_sync(0xffffffffu, q < s.chunks && s.pairs[min(q, s.chunks - 1) * s.chunk].x == key);
+      const int run = same == 0xffffffffu ? 32 : __ffs(~same) - 1;
+      heads += run;
+      if (run < 32) break;
+    }
+    if (heads > EG_LONG) {
+      if (lane == 0) {
+        const int k = atomicAdd(&long_count, 1);
+        long_runs[k][0] = c;
+        long_runs[k][1] = heads;
+      }
+      continue;
+    }
+    if (!live) continue;
     float f[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = 0.f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      const float4 x = part[w][lane], y = part[w][lane + 1];
-      f[0] += x.x; f[1] += x.y; f[2] += x.z; f[3] += x.w;
-      f[4] += y.x; f[5] += y.y; f[6] += y.z; f[7] += y.w;
-    }
+    add(s.tail, c, f);
+#pragma unroll 4
+    for (int h = 1; h <= heads; ++h) add(s.head, c + h, f);
     store_row8<DT>(s.out, static_cast<long long>(key) * s.ldo + col, f, s.scale, s.accumulate);
   }
+  __syncthreads();
+  for (int k = 0; k < long_count; ++k) {
+    const int c = long_runs[k][0], heads = long_runs[k][1];
+    const int per = (heads + 7) >> 3;
+    const int h0 = 1 + warp * per, h1 = min(h0 + per, heads + 1);
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = 0.f;
+    if (live) {
+      if (warp == 0) add(s.tail, c, f);
+#pragma unroll 4
+      for (int h = h0; h < h1; ++h) add(s.head, c + h, f);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) part[warp][j][lane] = f[j];
+    __syncthreads();
+    if (warp == 0 && live) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        f[j] = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) f[j] += part[w][j][lane];
+      }
+      store_row8<DT>(s.out, static_cast<long long>(s.pairs[c * s.chunk + s.chunk - 1].x) * s.ldo + col, f, s.scale, s.accumulate);
+    }
+    __syncthreads();
+  }
+}
+
+// Few tokens: a CTA per 256 columns finds every token's place by counting (equal tokens keep their order), its 32 warps sum
+// contiguous parts of the sorted list, and runs that cross from one warp to the next are joined through shared memory.
+constexpr int EG_FEW = 1024;
+
+struct EmbedGradFew {
+  const long long* tokens;
+  const void* dy;
+  long long ldy;
+  void* out;
+  long long ldo;
+  int n, rows, D, accumulate;
+  long long vocab_start, pad_idx;
+  float scale;
+};
+
+template <int DT>
+__global__ void __launch_bounds__(1024, 1) embed_grad_few_kernel(const EmbedGradFew s) {
+  extern __shared__ float few_smem[];
+  float* head = few_smem;               // [32][256]
+  float* tail = head + 32 * 256;        // [32][256]
+  uint32_t* keys = reinterpret_cast<uint32_t*>(tail + 32 * 256);  // [EG_FEW], padded with the largest number
+  uint32_t* skey = keys + EG_FEW;       // sorted
+  uint32_t* srow = skey + EG_FEW;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t none = static_cast<uint32_t>(s.rows);
+  dependents_wait();
+  uint32_t mine = 0xFFFFFFFFu;
+  if (tid < s.n) {
+    const long long t = s.tokens[tid];
+    const bool in = t != s.pad_idx && t >= s.vocab_start && t < s.vocab_start + s.rows;
+    mine = in ? static_cast<uint32_t>(t - s.vocab_start) : none;
+  }
+  keys[tid] = mine;
+  __syncthreads();
+  if (warp * 32 < s.n) {
+    int rank = 0;
+    const uint4* k4 = reinterpret_cast<const uint4*>(keys);
+    for (int i = 0; i < (s.n + 3) / 4; ++i) {  // below, or equal and earlier
+      const uint4 k = k4[i];
+      rank += (k.x < mine || (k.x == mine && 4 * i < tid)) + (k.y < mine || (k.y == mine && 4 * i + 1 < tid)) +
+              (k.z < mine || (k.z == mine && 4 * i + 2 < tid)) + (k.w < mine || (k.w == mine && 4 * i + 3 < tid));
+    }
+    if (tid < s.n) {
+      skey[rank] = mine;
+      srow[rank] = static_cast<uint32_t>(tid);
+    }
+  }
+  __syncthreads();
+  const int per = (s.n + 31) >> 5;
+  const int p0 = min(warp * per, s.n), p1 = min(p0 + per, s.n);
+  const int col = blockIdx.x * 256 + lane * 8;
+  const bool live = col < s.D;
+  const uint32_t prev = p0 > 0 ? skey[p0 - 1] : none, next = p1 < s.n ? skey[p1] : none;
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = 0.f;
+  uint32_t run = none;
+  bool first = true;
+  auto keep = [&](float* to) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) to[warp * 256 + j * 32 + lane] = f[j];
+  };
+  auto flush = [&](bool at_end) {
+    if (run == none) return;
+    if (first && run == prev) keep(head);
+    else if (at_end && run == next) keep(tail);
+    else if (live) store_row8<DT>(s.out, static_cast<long long>(run) * s.ldo + col, f, s.scale, s.accumulate);
+  };
+  for (int q0 = p0; q0 < p1; q0 += 8) {
+    Vec8<DT> v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (q0 + e < p1 && skey[q0 + e] != none && live) v[e].load(s.dy, static_cast<long long>(srow[q0 + e]) * s.ldy + col);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (q0 + e >= p1) break;
+      const uint32_t key = skey[q0 + e];
+      if (q0 + e > p0 && key != run) {
+        flush(false);
+        first = false;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = 0.f;
+      }
+      run = key;
+      if (key != none && live) v[e].add_to(f);
+    }
+  }
+  flush(true);
+  __syncthreads();
+  // the warp in whose part a crossing run begins adds the parts that follow
+  if (p1 > p0 && p1 < s.n) {
+    const uint32_t key = skey[p1 - 1];
+    const bool began_here = !(skey[p0] == key && prev == key);
+    if (key != none && next == key && began_here) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = tail[warp * 256 + j * 32 + lane];
+      for (int w = warp + 1; w < 32 && w * per < s.n && skey[w * per] == key; ++w) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] += head[w * 256 + j * 32 + lane];
+      }
+      if (live) store_row8<DT>(s.out, static_cast<long long>(key) * s.ldo + col, f, s.scale, s.accumulate);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(512) embed_grad_zero_kernel(uint4* out, long long vecs) {
+  dependents_launch();
+  const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
+  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < vecs; i += stride) out[i] = make_uint4(0u, 0u, 0u, 0u);
+}
+
+// A launch that may start while its predecessor in the stream drains (the kernel waits for it itself).
+template <typename... KArgs, typename... Args>
+static cudaError_t eg_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <int DT>
+static cudaError_t eg_launch_few(const EmbedGradFew& f, cudaStream_t stream) {
+  constexpr int smem = 2 * 32 * 256 * 4 + 3 * EG_FEW * 4;
+  const cudaError_t err = cudaFuncSetAttribute(embed_grad_few_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (err != cudaSuccess) return err;
+  const dim3 grid((f.D + 255) / 256);
+  if (!f.accumulate) return eg_launch(embed_grad_few_kernel<DT>, grid, dim3(1024), smem, stream, f);  // behind the fill
+  embed_grad_few_kernel<DT><<<grid, 1024, smem, stream>>>(f);
+  return cudaGetLastError();
+}
+
+template <int DT>
+static cudaError_t eg_launch_sums(const EmbedGradSum& su, unsigned blocks, dim3 join, cudaStream_t stream) {
+  const cudaError_t err = eg_launch(embed_grad_sum_kernel<DT>, dim3(blocks), dim3(256), 0, stream, su);
+  return err != cudaSuccess ? err : eg_launch(embed_grad_join_kernel<DT>, join, dim3(256), 0, stream, su);
 }
 
 static int eg_chunk(long long n, int D) {
@@ -330,6 +549,7 @@ static int eg_chunk(long long n, int D) {
 
 // Bytes of scratch (16-byte aligned) that msq_embed_grad_sorted needs for n tokens and D columns.
 extern "C" long long msq_embed_grad_workspace(int n, int D) {
+  if (n <= msq::EG_FEW) return 0;
   const long long chunk = msq::eg_chunk(n, D);
   const long long chunks = (n + chunk - 1) / chunk;
   return ((2LL * n * 8 + 255) & ~255LL) + 2LL * chunks * D * 4;
@@ -345,6 +565,21 @@ extern "C" int msq_embed_grad_sorted(const long long* tokens, const void* dy, lo
   if ((reinterpret_cast<uintptr_t>(dy) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15) return -4;
   if (!accumulate && ldo != D) return -4;
   if (n == 0 && accumulate) return 0;
+  int dev = 0, sms = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const long long vec_per_row = D / (dtype == 2 ? 4 : 8);
+  if (n <= EG_FEW) {
+    if (!accumulate) {
+      const long long vecs = rows * vec_per_row, want = (vecs + 2047) / 2048;
+      embed_grad_zero_kernel<<<static_cast<unsigned>(want < 4LL * sms ? want : 4LL * sms), 512, 0, stream>>>(static_cast<uint4*>(out), vecs);
+      if (cudaGetLastError() != cudaSuccess) return -11;
+      if (n == 0) return 0;
+    }
+    const EmbedGradFew f{tokens, dy, ldy, out, ldo, n, rows, D, accumulate, vocab_start, pad_idx, scale};
+    const cudaError_t err = dtype == 0 ? eg_launch_few<0>(f, stream) : dtype == 1 ? eg_launch_few<1>(f, stream) : eg_launch_few<2>(f, stream);
+    return err == cudaSuccess ? 0 : -11;
+  }
   EmbedGradSort so;
   so.tokens = tokens;
   so.buf[0] = static_cast<uint2*>(workspace);
@@ -357,19 +592,18 @@ extern "C" int msq_embed_grad_sorted(const long long* tokens, const void* dy, lo
   while (bits < 31 && (1LL << bits) <= rows) ++bits;  // keys 0 .. rows
   so.passes = (bits + 8) / 9;
   so.bits = (bits + so.passes - 1) / so.passes;
-  so.fill = accumulate ? nullptr : static_cast<uint4*>(out);
-  so.fill_vecs = accumulate ? 0 : static_cast<long long>(rows) * D / (dtype == 2 ? 4 : 8);
-  int dev = 0, sms = 0;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  // The sort takes about as long as filling 48 MB.
+  long long fill_first = accumulate ? 0 : (48LL << 20) / (vec_per_row * 16);
+  if (fill_first > rows) fill_first = accumulate ? 0 : rows;
+  so.fill = static_cast<uint4*>(out);
+  so.fill_vecs = fill_first * vec_per_row;
   const size_t smem = sizeof(int) * (EG_SORT_WARPS * EG_MAX_BINS + 2 * EG_MAX_BINS + 32);
   if (cudaFuncSetAttribute(embed_grad_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess) return -10;
   const long long fill_ctas = (so.fill_vecs + EG_SORT_THREADS * 4 - 1) / (EG_SORT_THREADS * 4);
   long long fill_clusters = (fill_ctas + EG_CLUSTER - 1) / EG_CLUSTER;
-  if (fill_clusters > 2 * sms / EG_CLUSTER) fill_clusters = 2 * sms / EG_CLUSTER;
+  if (fill_clusters > sms / EG_CLUSTER - 1) fill_clusters = sms / EG_CLUSTER - 1;
   embed_grad_sort_kernel<<<static_cast<unsigned>(EG_CLUSTER * (1 + fill_clusters)), EG_SORT_THREADS, smem, stream>>>(so);
   if (cudaGetLastError() != cudaSuccess) return -11;
-  if (n == 0) return 0;
   EmbedGradSum su;
   su.pairs = so.buf[(so.passes - 1) & 1];
   su.dy = dy; su.ldy = ldy; su.out = out; su.ldo = ldo;
@@ -381,16 +615,12 @@ extern "C" int msq_embed_grad_sorted(const long long* tokens, const void* dy, lo
   su.tail = su.head + static_cast<long long>(su.chunks) * D;
   su.accumulate = accumulate; su.scale = scale;
   const long long warps = static_cast<long long>(su.chunks) * su.slices;
-  const unsigned blocks = static_cast<unsigned>((warps + 7) / 8);
-  const dim3 join(static_cast<unsigned>(su.chunks), static_cast<unsigned>((D + 127) / 128));
-#define MSQ_EG(DT)                                                   \
-  do {                                                               \
-    embed_grad_sum_kernel<DT><<<blocks, 256, 0, stream>>>(su);       \
-    if (su.chunks > 1) embed_grad_join_kernel<DT><<<join, 256, 0, stream>>>(su); \
-  } while (0)
-  if (dtype == 0) MSQ_EG(0);
-  else if (dtype == 1) MSQ_EG(1);
-  else MSQ_EG(2);
-#undef MSQ_EG
-  return cudaGetLastError() == cudaSuccess ? 0 : -11;
+  su.fill_from = static_cast<int>(fill_first);
+  const long long left = accumulate ? 0 : rows - fill_first, want = (left + 255) / 256;
+  su.fill_blocks = static_cast<int>(want < sms ? want : sms);
+  const unsigned blocks = static_cast<unsigned>(su.fill_blocks + (warps + 7) / 8);
+  const dim3 join(static_cast<unsigned>((su.chunks + EG_JOIN - 1) / EG_JOIN), static_cast<unsigned>(su.slices));
+  const cudaError_t err = dtype == 0 ? eg_launch_sums<0>(su, blocks, join, stream) : dtype == 1 ? eg_launch_sums<1>(su, blocks, join, stream)
+                                                                                       : eg_launch_sums<2>(su, blocks, join, stream);
+  return err == cudaSuccess ? 0 : -11;
 }

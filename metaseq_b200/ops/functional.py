@@ -696,7 +696,8 @@ def embed_grad_sorted(tokens, dy, rows: int, scale: float = 1.0, pad_idx: int = 
         with _on_device(dy2):
             if out is None:
                 out = torch.empty((rows, D), dtype=dy2.dtype, device=dy2.device)
-            ws = torch.empty(max(16, lib.msq_embed_grad_workspace(n, D)), dtype=torch.uint8, device=dy2.device)
+            size = lib.msq_embed_grad_workspace(n, D)
+            ws = torch.empty(size, dtype=torch.uint8, device=dy2.device) if size else None
             rc = lib.msq_embed_grad_sorted(_lib.ptr(tok), _lib.ptr(dy2), dy2.stride(0), _lib.ptr(out),
                                            out.stride(0) if rows > 1 else D, n, rows, D, float(scale), int(vocab_start),
                                            int(pad_idx), int(accumulate), _lib.dtype_code(dy2.dtype), _lib.ptr(ws),
