@@ -23,6 +23,7 @@ constexpr int EG_CLUSTER = 8;
 constexpr int EG_SORT_THREADS = 1024;
 constexpr int EG_SORT_WARPS = EG_SORT_THREADS / 32;
 constexpr int EG_MAX_BINS = 512;
+constexpr long long EG_FILL_FIRST = 64;  // MB of a new table that are cleared beside the sort (16384 x 2048: 16 MB 81.8 us, 32 MB 80.5, 64 MB 79.0)
 
 __device__ __forceinline__ int eg_ld_remote(const int* p, uint32_t rank) {
   int v;
@@ -79,18 +80,31 @@ embed_grad_sort_kernel(const EmbedGradSort s) {
     }
     return __ldcg(s.buf[(pass - 1) & 1] + i);
   };
+  // Four pairs a lane at a time: their loads are in flight together, and where a warp's part is no longer than that (up to
+  // 32768 tokens) they stay in registers from the count to the placing.
+  const bool stay = per <= 128;
+  uint2 kv[4];
 
   for (int pass = 0; pass < s.passes; ++pass) {
     const int shift = pass * s.bits;
+    auto fetch = [&](int i0) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (i0 + 32 * q + lane < last) kv[q] = load(pass, i0 + 32 * q + lane);
+    };
     for (int b = lane; b < bins; b += 32) wh[b] = 0;
     __syncwarp();
-    for (int i0 = first; i0 < last; i0 += 32) {
-      const int i = i0 + lane;
-      const bool on = i < last;
-      const uint32_t d = on ? (load(pass, i).x >> shift) & (bins - 1) : 0xFFFFFFFFu;
-      const uint32_t peers = __match_any_sync(0xffffffffu, d);
-      if (on && lane == __ffs(peers) - 1) wh[d] += __popc(peers);
-      __syncwarp();
+    for (int i0 = first; i0 < last; i0 += 128) {
+      fetch(i0);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (i0 + 32 * q >= last) break;
+        const bool on = i0 + 32 * q + lane < last;
+        const uint32_t d = on ? (kv[q].x >> shift) & (bins - 1) : 0xFFFFFFFFu;
+        const uint32_t peers = __match_any_sync(0xffffffffu, d);
+        if (on && lane == __ffs(peers) - 1) wh[d] += __popc(peers);
+        __syncwarp();
+      }
     }
     __syncthreads();
     for (int b = tid; b < bins; b += EG_SORT_THREADS) {  // exclusive scan over this CTA's warps
@@ -129,21 +143,23 @@ embed_grad_sort_kernel(const EmbedGradSort s) {
     }
     __syncthreads();
     uint2* dst = s.buf[pass & 1];
-    for (int i0 = first; i0 < last; i0 += 32) {
-      const int i = i0 + lane;
-      const bool on = i < last;
-      const uint2 kv = on ? load(pass, i) : make_uint2(0u, 0u);
-      const uint32_t d = on ? (kv.x >> shift) & (bins - 1) : 0xFFFFFFFFu;
-      const uint32_t peers = __match_any_sync(0xffffffffu, d);
-      int at = 0;
-      if (on) at = base[d] + wh[d] + __popc(peers & ((1u << lane) - 1u));
-      __syncwarp();
-      if (on && lane == __ffs(peers) - 1) wh[d] += __popc(peers);
-      __syncwarp();
-      if (on) __stcg(dst + at, kv);
+    for (int i0 = first; i0 < last; i0 += 128) {
+      if (!stay) fetch(i0);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (i0 + 32 * q >= last) break;
+        const bool on = i0 + 32 * q + lane < last;
+        const uint32_t d = on ? (kv[q].x >> shift) & (bins - 1) : 0xFFFFFFFFu;
+        const uint32_t peers = __match_any_sync(0xffffffffu, d);
+        int at = 0;
+        if (on) at = base[d] + wh[d] + __popc(peers & ((1u << lane) - 1u));
+        __syncwarp();
+        if (on && lane == __ffs(peers) - 1) wh[d] += __popc(peers);
+        __syncwarp();
+        if (on) __stcg(dst + at, kv[q]);
+      }
     }
-    __threadfence();
-    cluster_sync_all();  // the pairs are in place, and nobody reads `total` of this pass any more
+    cluster_sync_all();  // (release and acquire at cluster scope) the pairs are in place, and nobody reads `total` of this pass any more
   }
 }
 
@@ -213,15 +229,19 @@ struct EmbedGradSum {
   int fill_from;
 };
 
-// Rows of a new table that no token names, 32 rows a warp at a time: every lane looks its row up in the sorted pairs.
+// Rows of a new table that no token names, EG_FILL_ROWS rows a warp at a time (few, so that the look-ups of some warps run
+// under the stores of others): every lane looks a row up in the sorted pairs.
+constexpr int EG_FILL_ROWS = 8;
+constexpr int EG_FILL_CTAS = 4;  // per SM (16384 x 2048: one 85.3 us, two 83.3, four 79.0)
+
 template <int DT>
 __device__ void embed_grad_fill(const EmbedGradSum& s) {
   constexpr int PER = DT == 2 ? 4 : 8;  // elements of 16 bytes
   const int lane = threadIdx.x & 31, vecs = s.D / PER;
-  const int warps = s.fill_blocks * 8;
   const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-  for (long long r0 = s.fill_from + 32LL * (blockIdx.x * 8 + (threadIdx.x >> 5)); r0 < s.rows; r0 += 32LL * warps) {
-    const long long row = r0 + lane;
+  const long long step = static_cast<long long>(EG_FILL_ROWS) * s.fill_blocks * 8;
+  for (long long r0 = s.fill_from + static_cast<long long>(EG_FILL_ROWS) * (blockIdx.x * 8 + (threadIdx.x >> 5)); r0 < s.rows; r0 += step) {
+    const long long row = r0 + (lane & (EG_FILL_ROWS - 1));
     bool clear = row < s.rows;
     if (clear) {
       int lo = 0, hi = s.n;  // first pair whose token is not below the row
@@ -232,7 +252,8 @@ __device__ void embed_grad_fill(const EmbedGradSum& s) {
       clear = lo == s.n || s.pairs[lo].x != static_cast<uint32_t>(row);
     }
     const unsigned mask = __ballot_sync(0xffffffffu, clear);
-    for (int k = 0; k < 32; ++k) {
+#pragma unroll
+    for (int k = 0; k < EG_FILL_ROWS; ++k) {
       if (!((mask >> k) & 1u)) continue;
       uint4* dst = static_cast<uint4*>(s.out) + (r0 + k) * vecs;
       for (int v = lane; v < vecs; v += 32) dst[v] = z;
@@ -592,8 +613,7 @@ extern "C" int msq_embed_grad_sorted(const long long* tokens, const void* dy, lo
   while (bits < 31 && (1LL << bits) <= rows) ++bits;  // keys 0 .. rows
   so.passes = (bits + 8) / 9;
   so.bits = (bits + so.passes - 1) / so.passes;
-  // The sort takes about as long as filling 48 MB.
-  long long fill_first = accumulate ? 0 : (48LL << 20) / (vec_per_row * 16);
+  long long fill_first = accumulate ? 0 : (EG_FILL_FIRST << 20) / (vec_per_row * 16);
   if (fill_first > rows) fill_first = accumulate ? 0 : rows;
   so.fill = static_cast<uint4*>(out);
   so.fill_vecs = fill_first * vec_per_row;
@@ -616,8 +636,8 @@ extern "C" int msq_embed_grad_sorted(const long long* tokens, const void* dy, lo
   su.accumulate = accumulate; su.scale = scale;
   const long long warps = static_cast<long long>(su.chunks) * su.slices;
   su.fill_from = static_cast<int>(fill_first);
-  const long long left = accumulate ? 0 : rows - fill_first, want = (left + 255) / 256;
-  su.fill_blocks = static_cast<int>(want < sms ? want : sms);
+  const long long left = accumulate ? 0 : rows - fill_first, want = (left + 8 * EG_FILL_ROWS - 1) / (8 * EG_FILL_ROWS);
+  su.fill_blocks = static_cast<int>(want < EG_FILL_CTAS * sms ? want : EG_FILL_CTAS * sms);
   const unsigned blocks = static_cast<unsigned>(su.fill_blocks + (warps + 7) / 8);
   const dim3 join(static_cast<unsigned>((su.chunks + EG_JOIN - 1) / EG_JOIN), static_cast<unsigned>(su.slices));
   const cudaError_t err = dtype == 0 ? eg_launch_sums<0>(su, blocks, join, stream) : dtype == 1 ? eg_launch_sums<1>(su, blocks, join, stream)
