@@ -15,6 +15,8 @@
 // All products are one kernel, the CTA-pair (cta_group::2) tcgen05 loop of gemm2_sm100.cu with eight epilogue warps:
 // 256 x 256 pair tiles, six TMA stages, two accumulators in tensor memory so that the epilogue of a tile runs under the
 // product of the next.
+#include <atomic>
+
 #include "sm100_pair.cuh"
 
 namespace msq {
@@ -128,18 +130,7 @@ lce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   const int pair = blockIdx.x >> 1;
   const int num_pairs = gridDim.x >> 1;
 
-  const int count = *p.count;
-  const int M = p.count_is == 1 ? count : p.M;
-  const int K = p.count_is == 2 ? count : p.K;
-  const int tiles_m = (M + 2 * LC_BM - 1) / (2 * LC_BM);
-  const int tiles_n = (p.N + LC_BN - 1) / LC_BN;
-  const int tiles = tiles_m * tiles_n;
-  const int m_cap = tiles_m * 2 * LC_BM;
-  const int splits = EPI == LCE_F32 && tiles > 0 ? lce_splits(tiles, p.count_is == 2 ? (K + LC_BK - 1) / LC_BK : p.split_k, p.slab_rows / m_cap, p.pairs) : 1;
-  const int num_items = tiles * splits;
-  const int k_total = (K + LC_BK - 1) / LC_BK;
-  const int k_per = (k_total + splits - 1) / splits;
-
+  // Everything up to dependents_wait may run while the predecessor drains.
   if (threadIdx.x == 0) {
     for (int s = 0; s < LC_STAGES; ++s) {
       mbar_init(&full_bar[s], 1);
@@ -150,29 +141,43 @@ lce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       mbar_init(&tempty_bar[b], 2 * LC_EPI_WARPS);
     }
     *abort_flag = 0;
-    if (rank == 0) {
-      // One decision for the pair: skip all work when an earlier launch left a timeout code behind.
-      const uint32_t skip = (p.status && *reinterpret_cast<volatile int*>(p.status) != 0) ? 1u : 0u;
-      *skip_flag = skip;
-      st_shared_cluster_u32(map_to_cta(smem_u32(const_cast<uint32_t*>(skip_flag)), 1), skip);
-    }
     mbar_fence_init();
     fence_proxy_async_smem();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
   }
-  __syncthreads();
-  cluster_sync_all();  // barriers of both CTAs are initialised, skip flag is in place
-  if (*skip_flag) return;
-
   if (warp == 1) {
     tmem_alloc_pair(tmem_slot, LC_TMEM_COLS);
     tmem_relinquish_pair();
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync_all();  // the barriers of both CTAs are initialised
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  dependents_launch();
+  dependents_wait();
+  if (threadIdx.x == 0 && rank == 0) {
+    // One decision for the pair: skip all work when an earlier launch left a timeout code behind.
+    const uint32_t skip = (p.status && *reinterpret_cast<volatile int*>(p.status) != 0) ? 1u : 0u;
+    *skip_flag = skip;
+    st_shared_cluster_u32(map_to_cta(smem_u32(const_cast<uint32_t*>(skip_flag)), 1), skip);
+  }
+  __syncthreads();
+  cluster_sync_all();
+
+  const bool skip_all = *skip_flag != 0;
+  const int count = skip_all ? 0 : *p.count;
+  const int M = p.count_is == 1 ? count : p.M;
+  const int K = p.count_is == 2 ? count : p.K;
+  const int tiles_m = skip_all ? 0 : (M + 2 * LC_BM - 1) / (2 * LC_BM);
+  const int tiles_n = (p.N + LC_BN - 1) / LC_BN;
+  const int tiles = tiles_m * tiles_n;
+  const int m_cap = tiles_m * 2 * LC_BM;
+  const int splits = EPI == LCE_F32 && tiles > 0 ? lce_splits(tiles, p.count_is == 2 ? (K + LC_BK - 1) / LC_BK : p.split_k, p.slab_rows / m_cap, p.pairs) : 1;
+  const int num_items = tiles * splits;
+  const int k_total = (K + LC_BK - 1) / LC_BK;
+  const int k_per = (k_total + splits - 1) / splits;
 
   if (warp == 0) {
     // ---------------------------------------------------------------- producer (both CTAs)
@@ -468,9 +473,10 @@ __global__ void __launch_bounds__(256) lce_compact_kernel(const LceCompact s) {
   __shared__ int red[8];
   __shared__ int place[LC_COMPACT_ROWS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  dependents_launch();
   const int r0 = blockIdx.x * LC_COMPACT_ROWS;
   int before = 0;
-#pragma unroll 4
+#pragma unroll 16
   for (int i = tid; i < r0; i += 256) before += s.target[i] != s.ignore;
   before = __reduce_add_sync(0xffffffffu, before);
   if (lane == 0) red[warp] = before;
@@ -498,13 +504,27 @@ __global__ void __launch_bounds__(256) lce_compact_kernel(const LceCompact s) {
     }
   }
   __syncthreads();
-  for (int k = warp; k < LC_COMPACT_ROWS; k += 8) {
-    const int at = place[k];
-    if (at < 0) continue;
-    const uint4* src = s.x + static_cast<long long>(r0 + k) * s.ldx;
-    uint4* dst = s.xc + static_cast<long long>(at) * s.vecs;
-#pragma unroll 4
-    for (int v = lane; v < s.vecs; v += 32) dst[v] = src[v];
+  // A warp's four rows side by side: eight loads a lane in flight.
+  const uint4* src[4];
+  uint4* dst[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int at = place[warp * 4 + k];
+    src[k] = at < 0 ? nullptr : s.x + static_cast<long long>(r0 + warp * 4 + k) * s.ldx;
+    dst[k] = at < 0 ? nullptr : s.xc + static_cast<long long>(at) * s.vecs;
+  }
+  for (int v = lane; v < s.vecs; v += 64) {
+    uint4 t[4][2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (src[k]) t[k][0] = src[k][v];
+      if (src[k] && v + 32 < s.vecs) t[k][1] = src[k][v + 32];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (dst[k]) dst[k][v] = t[k][0];
+      if (dst[k] && v + 32 < s.vecs) dst[k][v + 32] = t[k][1];
+    }
   }
   if (blockIdx.x == gridDim.x - 1) {
     if (tid == 0) {
@@ -513,8 +533,8 @@ __global__ void __launch_bounds__(256) lce_compact_kernel(const LceCompact s) {
     }
     const int stop = min(s.n, (end + 255) & ~255);
     const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-    uint4* dst = s.xc + static_cast<long long>(end) * s.vecs;
-    for (long long v = tid; v < static_cast<long long>(stop - end) * s.vecs; v += 256) dst[v] = z;
+    uint4* tail = s.xc + static_cast<long long>(end) * s.vecs;
+    for (long long v = tid; v < static_cast<long long>(stop - end) * s.vecs; v += 256) tail[v] = z;
   }
 }
 
@@ -534,44 +554,61 @@ struct LceMerge {
   float* total;
 };
 
-__global__ void __launch_bounds__(256) lce_merge_kernel(const LceMerge s) {
-  __shared__ float sm[8][32], ss[8][32];
+__global__ void __launch_bounds__(1024) lce_merge_kernel(const LceMerge s) {
+  __shared__ float sm[32][33], ss[32][33];
   __shared__ float red[32];
   __shared__ bool last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  dependents_launch();
+  dependents_wait();
   const int count = *s.count;
   const int row = blockIdx.x * 32 + lane;
+  auto fold = [](float& mx, float& sum, float m, float e) {  // parts without columns are (-inf, 0)
+    const float nm = fmaxf(mx, m);
+    sum = (sum == 0.f ? 0.f : sum * exp2f((mx - nm) * LC_LOG2E)) + (e == 0.f ? 0.f : e * exp2f((m - nm) * LC_LOG2E));
+    mx = nm;
+  };
   float mx = -INFINITY, sum = 0.f;
   if (row < count) {
-#pragma unroll 4
-    for (int i = warp; i < s.parts; i += 8) {
-      const float m = s.st_max[static_cast<long long>(i) * s.n + row], e = s.st_sum[static_cast<long long>(i) * s.n + row];
-      const float nm = fmaxf(mx, m);
-      sum = (sum == 0.f ? 0.f : sum * exp2f((mx - nm) * LC_LOG2E)) + (e == 0.f ? 0.f : e * exp2f((m - nm) * LC_LOG2E));
-      mx = nm;
+    for (int i0 = warp; i0 < s.parts; i0 += 128) {  // four parts' loads in flight
+      float m[4], e[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + 32 * k;
+        m[k] = i < s.parts ? s.st_max[static_cast<long long>(i) * s.n + row] : -INFINITY;
+        e[k] = i < s.parts ? s.st_sum[static_cast<long long>(i) * s.n + row] : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) fold(mx, sum, m[k], e[k]);
     }
   }
-  sm[warp][lane] = mx;
-  ss[warp][lane] = sum;
+  sm[lane][warp] = mx;
+  ss[lane][warp] = sum;
   __syncthreads();
-  float loss = 0.f;
-  if (warp == 0) {
-    if (row < count) {
+  // warp w folds row w of the 32: a butterfly over the warps' parts
+  mx = sm[warp][lane];
+  sum = ss[warp][lane];
 #pragma unroll
-      for (int w = 1; w < 8; ++w) {
-        const float m = sm[w][lane], e = ss[w][lane];
-        const float nm = fmaxf(mx, m);
-        sum = (sum == 0.f ? 0.f : sum * exp2f((mx - nm) * LC_LOG2E)) + (e == 0.f ? 0.f : e * exp2f((m - nm) * LC_LOG2E));
-        mx = nm;
-      }
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m = __shfl_xor_sync(0xffffffffu, mx, o), e = __shfl_xor_sync(0xffffffffu, sum, o);
+    fold(mx, sum, m, e);
+  }
+  const int mine = blockIdx.x * 32 + warp;
+  float loss = 0.f;
+  if (lane == 0) {
+    if (mine < count) {
       const float l2 = log2f(sum);
-      s.lse2[row] = fmaf(mx, LC_LOG2E, l2);
-      loss = mx - s.st_tgt[row] + l2 * LC_LN2;
-      s.loss[s.rows[row]] = loss;
-    } else if (row < ((s.n + 255) & ~255)) {
-      s.lse2[row] = INFINITY;
+      s.lse2[mine] = fmaf(mx, LC_LOG2E, l2);
+      loss = mx - s.st_tgt[mine] + l2 * LC_LN2;
+      s.loss[s.rows[mine]] = loss;
+    } else if (mine < ((s.n + 255) & ~255)) {
+      s.lse2[mine] = INFINITY;
     }
-    loss = warp_sum(loss);
+    red[warp] = loss;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    loss = warp_sum(red[lane]);
     if (lane == 0) {
       s.partial[blockIdx.x] = loss;
       __threadfence();
@@ -581,7 +618,7 @@ __global__ void __launch_bounds__(256) lce_merge_kernel(const LceMerge s) {
   __syncthreads();
   if (!last) return;
   float acc = 0.f;
-  for (int i = threadIdx.x; i < static_cast<int>(gridDim.x); i += 256) acc += __ldcg(s.partial + i);
+  for (int i = threadIdx.x; i < static_cast<int>(gridDim.x); i += 1024) acc += __ldcg(s.partial + i);
   acc = block_sum(acc, red);
   if (threadIdx.x == 0) *s.total = acc;
 }
@@ -606,6 +643,8 @@ struct LceFinish {
 
 __global__ void __launch_bounds__(256) lce_finish_kernel(const LceFinish s) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  dependents_launch();
+  dependents_wait();
   const int M = s.count ? *s.count : s.M;
   const float alpha = s.g ? s.alpha * *s.g : s.alpha;
   const int m_cap = (M + 2 * LC_BM - 1) / (2 * LC_BM) * (2 * LC_BM);
@@ -650,24 +689,55 @@ __global__ void __launch_bounds__(256) lce_finish_kernel(const LceFinish s) {
   }
 }
 
-static int lce_sms() {
-  int dev = 0, sms = 0;
+// Launches inside one call are chained: each may start while its predecessor drains, and waits for it before it touches
+// memory.  The first kernel of a call is launched the ordinary way.
+template <typename... KArgs, typename... Args>
+static int lce_chain(void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, bool chained, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = chained ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? 0 : -11;
+}
+
+static int lce_device() {
+  int dev = 0;
   cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return dev;
+}
+static int lce_sms() {
+  static std::atomic<int> known[64];
+  const int dev = lce_device();
+  int sms = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (sms == 0) {
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (dev < 64) known[dev].store(sms, std::memory_order_relaxed);
+  }
   return sms;
 }
 
 template <bool A_MN, bool B_MN, int EPI>
 static int lce_launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmC, const LceParams& p, int sms,
-                      cudaStream_t stream) {
+                      cudaStream_t stream, bool chained = true) {
   auto kern = lce_gemm_kernel<A_MN, B_MN, EPI>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, LC_SMEM) != cudaSuccess) return -10;
+  static std::atomic<unsigned long long> configured{0};  // a bit per device
+  const int dev = lce_device();
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
+  if (!(configured.load(std::memory_order_relaxed) & bit)) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, LC_SMEM) != cudaSuccess) return -10;
+    configured.fetch_or(bit, std::memory_order_relaxed);
+  }
   const long long items = static_cast<long long>((p.M + 2 * LC_BM - 1) / (2 * LC_BM)) * ((p.N + LC_BN - 1) / LC_BN) * (EPI == LCE_F32 ? 32 : 1);
   long long pairs = sms / 2;
   if (pairs > items) pairs = items;
   if (pairs <= 0) return 0;
-  kern<<<static_cast<unsigned>(2 * pairs), LC_THREADS, LC_SMEM, stream>>>(tmA, tmB, tmC, p);
-  return cudaGetLastError() == cudaSuccess ? 0 : -11;
+  return lce_chain(kern, static_cast<unsigned>(2 * pairs), LC_THREADS, LC_SMEM, stream, chained, tmA, tmB, tmC, p);
 }
 
 // Tensor map of an output: tiles of 32 rows x 128 bytes.
@@ -829,8 +899,7 @@ extern "C" int msq_lce_fwd(const void* x, long long ldx, const void* w, long lon
   LceMerge m;
   m.st_max = st_max; m.st_sum = st_sum; m.st_tgt = st_tgt; m.parts = parts; m.n = n;
   m.rows = sv.rows; m.count = sv.count; m.lse2 = sv.lse2; m.loss = loss; m.partial = partial; m.ticket = ticket; m.total = total;
-  lce_merge_kernel<<<(n + 255) / 256 * 8, 256, 0, stream>>>(m);
-  return cudaGetLastError() == cudaSuccess ? 0 : -11;
+  return lce_chain(lce_merge_kernel, (n + 255) / 256 * 8, 1024, 0, stream, true, m);
 }
 
 // dx [n, D] (0 in ignored rows) and dw [V, D] (added to what is there when `accumulate`), both times g[0]; either may be
@@ -871,7 +940,7 @@ extern "C" int msq_lce_bwd(const void* w, long long ldw, const long long* target
     if ((rc = lce_out_map(&tmP, P, n, pv, q.piece, false, bf16))) return rc;
     p.M = n; p.N = pv; p.K = D; p.count_is = 1;
     p.target = sv.tgt; p.v0 = v0; p.lse2 = sv.lse2; p.p_log2 = p_log2;
-    if ((rc = lce_launch<false, false, LCE_PROB>(tmXk, tmW, tmP, p, sms, stream))) return rc;
+    if ((rc = lce_launch<false, false, LCE_PROB>(tmXk, tmW, tmP, p, sms, stream, v0 > 0))) return rc;
     if (dx) {
       if ((rc = make_tmap_2d(&tmPk, P, n, pv, q.piece, LC_BM, bf16))) return rc;
       if ((rc = make_tmap_2d(&tmWmn, wp, pv, D, ldw, LC_BK, bf16))) return rc;
@@ -891,7 +960,7 @@ extern "C" int msq_lce_bwd(const void* w, long long ldw, const long long* target
         f.acc = dw32; f.pairs = sms / 2; f.slab_rows = p.slab_rows; f.split_count = sv.count; f.D = D; f.M = pv;
         f.out = dwp; f.ldo = lddw; f.g = g; f.alpha = alpha; f.accumulate = accumulate; f.bf16 = bf16;
         const int blocks = (pv + 7) / 8;
-        lce_finish_kernel<<<blocks < 8 * sms ? blocks : 8 * sms, 256, 0, stream>>>(f);
+        if ((rc = lce_chain(lce_finish_kernel, blocks < 8 * sms ? blocks : 8 * sms, 256, 0, stream, true, f))) return rc;
       } else {
         if ((rc = lce_out_map(&tmOut, dwp, pv, D, lddw, false, bf16))) return rc;
         p.accumulate = accumulate; p.out = dwp; p.ldo = lddw; p.g = g;
@@ -905,7 +974,7 @@ extern "C" int msq_lce_bwd(const void* w, long long ldw, const long long* target
     f.rows = sv.rows; f.count = sv.count; f.target = target; f.ignore = ignore;
     f.out = static_cast<uint16_t*>(dx); f.ldo = lddx; f.g = g; f.alpha = alpha; f.bf16 = bf16;
     const int blocks = (n + 7) / 8;
-    lce_finish_kernel<<<blocks < 8 * sms ? blocks : 8 * sms, 256, 0, stream>>>(f);
+    if ((rc = lce_chain(lce_finish_kernel, blocks < 8 * sms ? blocks : 8 * sms, 256, 0, stream, true, f))) return rc;
   }
-  return cudaGetLastError() == cudaSuccess ? 0 : -11;
+  return 0;
 }

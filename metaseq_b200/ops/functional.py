@@ -985,7 +985,8 @@ def linear_cross_entropy_fwd(x, weight, target, ignore_index: int):
     makes the loss of its token NaN.  Logits, sums and statistics are fp32."""
     _linear_ce_check(x, weight, target)
     V, D = weight.shape
-    x2, tgt = x.reshape(-1, D), target.reshape(-1).contiguous()
+    x2 = x if x.dim() == 2 else x.reshape(-1, D)
+    tgt = (target if target.dim() == 1 else target.reshape(-1)).contiguous()
     n = tgt.numel()
     ensure_operand_ready(weight)
     if _linear_ce_kernel_ok(x2, weight):
@@ -996,9 +997,9 @@ def linear_cross_entropy_fwd(x, weight, target, ignore_index: int):
             loss = torch.empty(n + 1, dtype=torch.float32, device=x2.device)
             saved = torch.empty(lib.msq_lce_saved_bytes(n, V, D), dtype=torch.uint8, device=x2.device)
             ws = torch.empty(lib.msq_lce_fwd_bytes(n, V, D), dtype=torch.uint8, device=x2.device)
-            rc = lib.msq_lce_fwd(_lib.ptr(x2), x2.stride(0), _lib.ptr(weight), weight.stride(0), _lib.ptr(tgt), n, V, D,
-                                 int(ignore_index), _lib.ptr(loss), loss.data_ptr() + 4 * n, _lib.ptr(saved),
-                                 _lib.ptr(ws), _bf(x2), _lib.ptr(_lib.status_word(x2.device)), _lib.stream_ptr())
+            rc = lib.msq_lce_fwd(x2.data_ptr(), x2.stride(0), weight.data_ptr(), weight.stride(0), tgt.data_ptr(), n, V, D,
+                                 int(ignore_index), loss.data_ptr(), loss.data_ptr() + 4 * n, saved.data_ptr(),
+                                 ws.data_ptr(), _bf(x2), _lib.status_word(x2.device).data_ptr(), _lib.stream_ptr())
         _lib.check_rc(rc, "msq_lce_fwd")
         return loss[:n].view(target.shape), loss[n], (saved,)
     if x2.is_cuda and x2.dtype in (torch.float16, torch.bfloat16) and n:
