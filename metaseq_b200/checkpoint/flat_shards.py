@@ -135,6 +135,17 @@ def reshard_optimizer_state(states: Sequence[Dict[str, Any]], new_rank: int, new
             if torch.is_tensor(val) and val.dim() > 0 and key is not None and val.numel() == states[0]["model"][key].numel():
                 total = unpadded_numel(mds[0][key])
                 pieces = [s["last_optimizer_state"]["state"][idx] for s in states]
+                plain = {"exp_avg_8": "exp_avg", "exp_avg_sq_root_8": "exp_avg_sq"}.get(name)
+                if plain is not None:
+                    from metaseq_b200.ops.functional import adamw8_decode
+
+                    # moments in 8 bits, one scale per 256 values of a shard, the second as its root: joined as fp32 as well
+                    tensors = [adamw8_decode(pc[name].to(torch.float8_e4m3fn), pc[name + "_scale"].float()) for pc in pieces]
+                    if plain == "exp_avg_sq":
+                        tensors = [t.square() for t in tensors]
+                    vec = logical_vector(tensors, [m[key].get("padding", 0) for m in mds], total)
+                    entry[plain], _ = slice_for_rank(vec, new_rank, new_world)
+                    continue
                 if name + "_scale" in st:
                     # moments stored as scaled fp16: every shard has its own scale, so they are joined as fp32 and
                     # the optimizer compresses them again after its next step

@@ -10,7 +10,7 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as TF
 
-from metaseq_b200.dataclass.configs import MetaseqDataclass
+from metaseq_b200.dataclass.configs import MetaseqDataclass, opt
 from metaseq_b200.logging import metrics
 from metaseq_b200.ops import autograd as ops_ag
 from metaseq_b200.ops import functional as ops_f
@@ -19,9 +19,14 @@ from . import register_criterion
 from .base_criterion import BaseCriterion
 
 
+LOGITS_FREE_HELP = ("compute the loss from the final features in pieces of the vocabulary: the logits of all tokens are "
+                    "never stored and the backward pass computes them again (less memory, about a third more work in the "
+                    "projection; ignored targets are skipped)")
+
+
 @dataclass
 class CrossEntropyCriterionConfig(MetaseqDataclass):
-    pass
+    logits_free: bool = opt(False, LOGITS_FREE_HELP)
 
 
 def nll_loss_sum(logits, target, ignore_index, row_stats=None):
@@ -59,12 +64,17 @@ def nll_loss(lprobs, target, ignore_index=None, reduction: str = "mean"):
 
 @register_criterion("cross_entropy", dataclass=CrossEntropyCriterionConfig)
 class CrossEntropyCriterion(BaseCriterion):
-    def __init__(self, task):
+    def __init__(self, task, logits_free: bool = False):
         super().__init__(task)
+        self.logits_free = logits_free
 
     def forward(self, model, sample, reduce=True):
-        net_output = model(**sample["net_input"])
-        loss, _ = self.compute_loss(model, net_output, sample, reduce=reduce)
+        if self.logits_free:
+            net_output = model(**sample["net_input"], loss_target=sample["target"], loss_ignore_index=self.padding_idx)
+            loss = net_output[0]
+        else:
+            net_output = model(**sample["net_input"])
+            loss, _ = self.compute_loss(model, net_output, sample, reduce=reduce)
         sample_size = sample["ntokens"]
         logging_output = {
             "loss": loss.data,

@@ -9,35 +9,43 @@ from dataclasses import dataclass
 
 import torch
 
-from metaseq_b200.dataclass.configs import MetaseqDataclass
+from metaseq_b200.dataclass.configs import MetaseqDataclass, opt
 from metaseq_b200.logging import metrics
 from metaseq_b200.parallel import mpu
 from metaseq_b200.parallel.cross_entropy import vocab_parallel_cross_entropy
 
 from . import register_criterion
 from .base_criterion import BaseCriterion
-from .cross_entropy import _ppl, nll_loss_sum
+from .cross_entropy import LOGITS_FREE_HELP, _ppl, nll_loss_sum
 
 
 @dataclass
 class VocabParallelCrossEntropyConfig(MetaseqDataclass):
-    pass
+    logits_free: bool = opt(False, LOGITS_FREE_HELP)
 
 
 @register_criterion("vocab_parallel_cross_entropy", dataclass=VocabParallelCrossEntropyConfig)
 class VocabParallelCrossEntropyCriterion(BaseCriterion):
-    def __init__(self, task):
+    def __init__(self, task, logits_free: bool = False):
         super().__init__(task)
+        if logits_free and mpu.get_tensor_model_parallel_world_size() > 1:
+            raise ValueError("--logits-free needs the whole vocabulary on one rank (--model-parallel-size 1)")
+        self.logits_free = logits_free
 
     def forward(self, model, sample, reduce=True):
         target = sample["target"]
         # Non-pad target count comes from the collater (computed on the host before the batch is
         # copied to the device), so no device-to-host sync is needed here.
         has_pad = True
-        net_output = model(**sample["net_input"])
+        if self.logits_free:
+            net_output = model(**sample["net_input"], loss_target=target, loss_ignore_index=self.padding_idx)
+        else:
+            net_output = model(**sample["net_input"])
         logits = net_output[0]
         row_stats = getattr(logits, "_msq_row_stats", None)  # left by the logits product's epilogue
-        if mpu.get_tensor_model_parallel_world_size() == 1:
+        if self.logits_free:
+            loss = logits
+        elif mpu.get_tensor_model_parallel_world_size() == 1:
             loss = nll_loss_sum(logits.reshape(-1, logits.size(-1)), target.reshape(-1), self.padding_idx, row_stats)
         else:
             from metaseq_b200.parallel.cross_entropy import fused_vocab_parallel_cross_entropy_ok

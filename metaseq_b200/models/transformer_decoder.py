@@ -249,10 +249,14 @@ class ModelParallelTransformerDecoder(IncrementalDecoder):
 
     # ---------------------------------------------------------------- forward
     def forward(self, prev_output_tokens, src_lengths=None, incremental_state=None, features_only: bool = False,
-                self_attn_padding_mask=None, **unused):
+                self_attn_padding_mask=None, loss_target=None, loss_ignore_index: int = -100, **unused):
+        """``loss_target`` (``[B, T]``): the first result is then the cross entropy summed over the targets that are not
+        ``loss_ignore_index``, computed from the final features without the logits (``output_loss``)."""
         x, extra = self.extract_features(prev_output_tokens, incremental_state=incremental_state,
                                          self_attn_padding_mask=self_attn_padding_mask)
-        if not features_only:
+        if loss_target is not None:
+            x = self.output_loss(x, loss_target, loss_ignore_index, norm_sums=extra.get("norm_sums"))
+        elif not features_only:
             x = self.output_layer(x, bt=extra["bt"], norm_sums=extra.get("norm_sums"))
         return x, extra
 
@@ -333,6 +337,17 @@ class ModelParallelTransformerDecoder(IncrementalDecoder):
         if row_stats is not None:
             logits._msq_row_stats = row_stats
         return logits
+
+    def output_loss(self, features, target, ignore_index: int, norm_sums=None):
+        """Summed cross entropy of the projection to the vocabulary, in pieces of the vocabulary: the ``[tokens, V]``
+        logits are never stored (``ops.autograd.linear_cross_entropy_sum``).  Needs the whole vocabulary on this rank."""
+        if mpu.get_tensor_model_parallel_world_size() > 1:
+            raise ValueError("the loss without logits needs the whole vocabulary on one rank (tensor parallel size 1)")
+        if norm_sums is not None:
+            with torch.no_grad():
+                norm_sums["actv"] = torch.linalg.vector_norm(features.detach(), dim=-1, dtype=torch.float32).sum()
+        w = self.output_projection.weight
+        return ops_ag.linear_cross_entropy_sum(features.to(w.dtype), w, target.reshape(features.shape[:-1]), ignore_index)
 
     def max_positions(self):
         if self.embed_positions is None:

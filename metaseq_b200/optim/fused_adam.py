@@ -19,10 +19,11 @@ class FusedAdamV1(Adam):
     the gradients (combined loss scale and clipping).  Explicit ``grads`` are copied onto ``.grad`` first."""
 
     def __init__(self, params, lr=1e-3, bias_correction=True, betas=(0.9, 0.999), eps=1e-8, eps_inside_sqrt=False,
-                 weight_decay=0.0, max_grad_norm=0.0, amsgrad=False, use_fp16_stats=False):
+                 weight_decay=0.0, max_grad_norm=0.0, amsgrad=False, use_fp16_stats=False, use_fp8_stats=False):
         if amsgrad:
             raise RuntimeError("FusedAdam does not support the AMSGrad variant.")
-        super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, use_fp16_stats=use_fp16_stats)
+        super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, use_fp16_stats=use_fp16_stats,
+                         use_fp8_stats=use_fp8_stats)
         self.max_grad_norm = max_grad_norm
 
     def step(self, closure=None, grads=None, scale: float = 1.0, grad_norms=None, ctrl: Optional[torch.Tensor] = None):
