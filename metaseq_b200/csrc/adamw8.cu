@@ -391,14 +391,14 @@ struct Adam8Hyper {
 };
 
 template <int PDT, int GDT, int COUNT>
-static int launch_adamw8(const long long* rec, int count, long long block0, int tile_blocks, const Adam8Hyper& h, cudaStream_t stream) {
+static int launch_adamw8(const unsigned long long* ptrs, const long long* sizes, int count, long long block0, int tile_blocks, const Adam8Hyper& h, cudaStream_t stream) {
   Adam8Args<COUNT> a;
   a.count = count;
   a.tile_blocks = tile_blocks;
   a.block0 = block0;
   long long tiles = 0, blocks = 0;
   for (int i = 0; i < count; ++i) {
-    const long long* q = rec + 7 * i;
+    const unsigned long long* q = ptrs + 6 * i;
     Adam8Tensor& t = a.t[i];
     t.p = reinterpret_cast<void*>(q[0]);
     t.g = reinterpret_cast<const void*>(q[1]);
@@ -406,7 +406,7 @@ static int launch_adamw8(const long long* rec, int count, long long block0, int 
     t.ms = reinterpret_cast<float*>(q[3]);
     t.r = reinterpret_cast<uint8_t*>(q[4]);
     t.rs = reinterpret_cast<float*>(q[5]);
-    t.n = q[6];
+    t.n = sizes[i];
     t.first_tile = static_cast<int>(tiles);
     t.first_block = static_cast<int>(blocks);
     const long long nb = (t.n + A8_BLOCK - 1) / A8_BLOCK;
@@ -429,9 +429,9 @@ static int launch_adamw8(const long long* rec, int count, long long block0, int 
 
 }  // namespace msq
 
-// `records`: host memory, seven 64-bit words per tensor: {p, g, codes of m, scales of m, codes of r, scales of r, elements}.
-// Scales: one fp32 per block of 256 elements.  Tensors with no elements are allowed.
-extern "C" int msq_adamw8_multi(const long long* records, int count, int p_dtype, int g_dtype, float beta1, float omb1,
+// Host memory: `ptrs` holds six addresses per tensor, {p, g, codes of m, scales of m, codes of r, scales of r}, `sizes` its
+// elements.  Scales: one fp32 per block of 256 elements.  Tensors with no elements are allowed.
+extern "C" int msq_adamw8_multi(const unsigned long long* ptrs, const long long* sizes, int count, int p_dtype, int g_dtype, float beta1, float omb1,
                                 float beta2, float omb2, float eps, float decay, float step_size, unsigned long long seed,
                                 const float* ctrl, cudaStream_t stream) {
   using namespace msq;
@@ -441,14 +441,14 @@ extern "C" int msq_adamw8_multi(const long long* records, int count, int p_dtype
   for (int at = 0; at < count;) {
     const int n = count - at < MANY ? count - at : MANY;
     long long blocks = 0;
-    for (int i = 0; i < n; ++i) blocks += (records[7 * (at + i) + 6] + A8_BLOCK - 1) / A8_BLOCK;
+    for (int i = 0; i < n; ++i) blocks += (sizes[at + i] + A8_BLOCK - 1) / A8_BLOCK;
     // A CTA's tile: long ones save the start-up of the copies (403M elements: 32 blocks 866 us, 128 blocks 831 us), short
     // ones spread small lists over the SMs (one block per warp at the least).
     const int tile_blocks = blocks >= 2 * 3 * 148 * 128 ? 128 : blocks >= 148 * 8 * 32 ? 32 : 8;
     int rc = -2;
 #define MSQ_A8(PD, GD)                                                                                      \
-  rc = n <= FEW ? launch_adamw8<PD, GD, FEW>(records + 7 * at, n, block0, tile_blocks, h, stream)            \
-                : launch_adamw8<PD, GD, MANY>(records + 7 * at, n, block0, tile_blocks, h, stream)
+  rc = n <= FEW ? launch_adamw8<PD, GD, FEW>(ptrs + 6 * at, sizes + at, n, block0, tile_blocks, h, stream)            \
+                : launch_adamw8<PD, GD, MANY>(ptrs + 6 * at, sizes + at, n, block0, tile_blocks, h, stream)
     if (p_dtype == 0 && g_dtype == 0) MSQ_A8(0, 0);
     else if (p_dtype == 1 && g_dtype == 1) MSQ_A8(1, 1);
     else if (p_dtype == 2 && g_dtype == 0) MSQ_A8(2, 0);

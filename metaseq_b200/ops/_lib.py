@@ -167,7 +167,7 @@ _OPTIONAL = {
     "msq_gemm2_rowstats": [P, P, P, I, I, I, L, L, L, I, I, I, P, P, P, I, P, P, P],
     "msq_ce_merge_rowstats": [P, P, I, I, P, L, P, I, L, P, P, I, I, I, ctypes.c_uint, I, P],
     "msq_vp_ce_finish_exchanged": [P, L, P, P, I, I, ctypes.c_uint, P, I, I, L, L, F, I, P, P],
-    "msq_adamw8_multi": [P, I, I, I, F, F, F, F, F, F, F, ctypes.c_ulonglong, P, P],
+    "msq_adamw8_multi": [P, P, I, I, I, F, F, F, F, F, F, F, ctypes.c_ulonglong, P, P],
     "msq_lce_fwd": [P, L, P, L, P, I, I, I, L, P, P, P, P, I, P, P],
     "msq_lce_bwd": [P, L, P, I, I, I, L, P, P, P, L, P, L, I, P, I, P, P],
     "msq_embed_grad_sorted": [P, P, L, P, L, I, I, I, F, L, L, I, I, P, P],

@@ -12,8 +12,9 @@ cuBLAS + unfused-ops baseline the kernels are compared against).
 """
 from __future__ import annotations
 
+import array
 import contextlib
-import ctypes
+import itertools
 import logging
 import math
 import operator
@@ -1365,29 +1366,28 @@ _ADAMW8_GRADS = {torch.float16: (torch.float16, torch.float32), torch.bfloat16: 
 _DTYPE_OF, _DEVICE_OF = operator.attrgetter("dtype"), torch.Tensor.get_device  # -1 off the GPU
 
 
-def _adamw8_check(columns):
-    """Refuses lists that the update cannot take.  ``columns``: the parameters, gradients, codes and scales, a tuple
-    each.  Whole lists are looked over at once: a list of a few hundred tensors is common."""
-    p, g, m, ms, r, rs = columns
-    pdt, gdt = set(map(_DTYPE_OF, p)), set(map(_DTYPE_OF, g))
-    if len(pdt) != 1 or len(gdt) != 1 or next(iter(gdt)) not in _ADAMW8_GRADS.get(next(iter(pdt)), ()):
-        raise ValueError("adamw8_step_multi: all parameters share one type, all gradients one type that goes with it "
-                         f"(the parameters' or fp32; any with fp32 parameters), not {pdt} with {gdt}")
-    if set(map(_DTYPE_OF, m)) | set(map(_DTYPE_OF, r)) != {torch.float8_e4m3fn}:
+def _adamw8_check(flat):
+    """Refuses lists that the update cannot take; returns the parameters' sizes.  ``flat``: the items' tensors one after
+    the other.  A list of a few hundred tensors is common, so every property is read off all of them in one go."""
+    dtypes = list(map(_DTYPE_OF, flat))
+    n, pdt, gdt = len(flat) // 6, dtypes[0], dtypes[1]
+    if dtypes[0::6].count(pdt) != n or dtypes[1::6].count(gdt) != n or gdt not in _ADAMW8_GRADS.get(pdt, ()):
+        raise ValueError("adamw8_step_multi: all parameters share one type, all gradients one type that goes with it (the "
+                         f"parameters' or fp32; any with fp32 parameters), not {set(dtypes[0::6])} with {set(dtypes[1::6])}")
+    if dtypes[2::6].count(torch.float8_e4m3fn) != n or dtypes[4::6].count(torch.float8_e4m3fn) != n:
         raise ValueError("adamw8_step_multi: the codes must be float8_e4m3fn (adamw8_state)")
-    if set(map(_DTYPE_OF, ms)) | set(map(_DTYPE_OF, rs)) != {torch.float32}:
+    if dtypes[3::6].count(torch.float32) != n or dtypes[5::6].count(torch.float32) != n:
         raise ValueError("adamw8_step_multi: the scales must be fp32 (adamw8_state)")
-    flat = [t for column in columns for t in column]
-    devices = set(map(_DEVICE_OF, flat))
-    if len(devices) != 1 or (devices == {-1} and len({t.device for t in flat}) != 1):
+    devices = list(map(_DEVICE_OF, flat))
+    if devices.count(devices[0]) != 6 * n or (devices[0] < 0 and len({t.device for t in flat}) != 1):
         raise ValueError("adamw8_step_multi: tensors on different devices")
     if not all(map(torch.Tensor.is_contiguous, flat)):
         raise ValueError("adamw8_step_multi: tensors must be contiguous")
-    numel = torch.Tensor.numel
-    sizes = list(map(numel, p))
-    if not sizes == list(map(numel, g)) == list(map(numel, m)) == list(map(numel, r)):
+    numel = list(map(torch.Tensor.numel, flat))
+    sizes = numel[0::6]
+    if not sizes == numel[1::6] == numel[2::6] == numel[4::6]:
         raise ValueError("adamw8_step_multi: a parameter, its gradient and its codes differ in size")
-    if not [-(-n // ADAMW8_BLOCK) for n in sizes] == list(map(numel, ms)) == list(map(numel, rs)):
+    if not [(k + ADAMW8_BLOCK - 1) // ADAMW8_BLOCK for k in sizes] == numel[3::6] == numel[5::6]:
         raise ValueError(f"adamw8_step_multi: one scale per block of {ADAMW8_BLOCK} elements is wanted (adamw8_state)")
     return sizes
 
@@ -1405,28 +1405,25 @@ def adamw8_step_multi(items, *, lr, beta1, beta2, eps, weight_decay, step, seed,
     items = list(items)
     if not items:
         return
-    columns = tuple(zip(*items))
-    if len(columns) != 6:
+    if set(map(len, items)) != {6}:
         raise ValueError("adamw8_step_multi: items are (p, g, m codes, m scales, r codes, r scales)")
-    sizes = _adamw8_check(columns)
+    flat = list(itertools.chain.from_iterable(items))
+    sizes = _adamw8_check(flat)
     if step < 1:
         raise ValueError(f"adamw8_step_multi: the first step is 1, not {step}")
     seed = int(seed)
     if not 0 <= seed < 1 << 64:
         raise ValueError("adamw8_step_multi: seed must be in [0, 2^64)")
-    p0, g0 = columns[0][0], columns[1][0]
+    p0, g0 = flat[0], flat[1]
     if ctrl is not None and (ctrl.dtype != torch.float32 or ctrl.device != p0.device or ctrl.numel() < 2
                              or not ctrl.is_contiguous()):
         raise ValueError("adamw8_step_multi: ctrl is the fp32 control block of clip_decision on the tensors' device")
     step_size = lr * (1.0 - beta2 ** step) ** 0.5 / (1.0 - beta1 ** step)
     decay, omb1, omb2 = lr * weight_decay, 1.0 - beta1, 1.0 - beta2
     if _float_kernels(p0):
-        words = [None] * (7 * len(items))
-        for k, column in enumerate(columns):
-            words[k::7] = map(torch.Tensor.data_ptr, column)
-        words[6::7] = sizes
+        pointers, counts = array.array("Q", map(torch.Tensor.data_ptr, flat)), array.array("q", sizes)
         with _on_device(p0):
-            rc = _lib.kernels().msq_adamw8_multi((ctypes.c_longlong * len(words))(*words), len(items),
+            rc = _lib.kernels().msq_adamw8_multi(pointers.buffer_info()[0], counts.buffer_info()[0], len(items),
                                                  _lib.dtype_code(p0.dtype), _lib.dtype_code(g0.dtype), beta1, omb1, beta2,
                                                  omb2, eps, decay, step_size, seed, _lib.ptr(ctrl), _lib.stream_ptr())
         _lib.check_rc(rc, "msq_adamw8_multi")
