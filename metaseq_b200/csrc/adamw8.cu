@@ -16,7 +16,7 @@
 // scale does, so a value that does not change is stored without another draw.  A root above zero is never stored as
 // zero: next to a live first moment a zero denominator would turn into a step of m / eps.
 //
-// One warp per block of 256: every lane takes eight values of p, g, m and r from a four-stage ring of asynchronous copies, the
+// One warp per block of 256: every lane takes eight values of p, g, m and r from a ring of asynchronous copies, the
 // block's largest magnitudes are found with two warp reductions, and everything is written in the same pass: 10 bytes a
 // parameter for 16-bit p and g.  What bounds it is instruction issue, about 50 per element (403M bf16 parameters: 0.82 ms,
 // 4.9 TB/s; the bytes alone would take 0.63 ms).
@@ -231,9 +231,11 @@ struct A8Slot {
   uint2 m[32], r[32];
   float ms, rs, pad[2];
 };
-constexpr int A8_STAGES = 4;
+// Ring stages of a warp: three where a slot is larger, so that three CTAs fit on an SM.
 template <int PDT, int GDT>
-constexpr int a8_smem() { return 8 * A8_STAGES * static_cast<int>(sizeof(A8Slot<PDT, GDT>)); }
+__host__ __device__ constexpr int a8_stages() { return PDT == 2 || GDT == 2 ? 3 : 4; }
+template <int PDT, int GDT>
+constexpr int a8_smem() { return 8 * a8_stages<PDT, GDT>() * static_cast<int>(sizeof(A8Slot<PDT, GDT>)); }
 
 template <int DT>
 __device__ __forceinline__ void a8_store8(void* base, long long i, const uint64_t (&f)[4]) {
@@ -263,7 +265,7 @@ __device__ __forceinline__ void a8_store1(void* base, long long i, float v) {
 }
 
 template <int PDT, int GDT, int COUNT>
-__global__ void __launch_bounds__(256, PDT == 2 || GDT == 2 ? 2 : 3) adamw8_kernel(const __grid_constant__ Adam8Args<COUNT> a) {
+__global__ void __launch_bounds__(256, 3) adamw8_kernel(const __grid_constant__ Adam8Args<COUNT> a) {
   extern __shared__ uint4 a8_shared[];
   if (a.ctrl && a.ctrl[1] != 0.f) return;  // overflow: parameters and moments stay as they are
   const Adam8Consts c{a.ctrl ? a.ctrl[0] : 1.f, a.beta1, a.omb1, a.beta2, a.omb2, a.eps, a.decay, a.step_size, a.minus_zero};
@@ -289,8 +291,8 @@ __global__ void __launch_bounds__(256, PDT == 2 || GDT == 2 ? 2 : 3) adamw8_kern
     // ahead left the warps waiting for memory).  Every lane copies and reads its own bytes; only the scales are shared.
     const long long whole = min(b1, t.n / A8_BLOCK);
     const int iters = b < whole ? static_cast<int>((whole - b + 7) >> 3) : 0;
-    constexpr int PB = PDT == 2 ? 4 : 2, GB = GDT == 2 ? 4 : 2, STEP = 8 * A8_BLOCK;  // elements from one of the warp's blocks to the next
-    A8Slot<PDT, GDT>* slots = reinterpret_cast<A8Slot<PDT, GDT>*>(a8_shared) + warp * A8_STAGES;
+    constexpr int STAGES = a8_stages<PDT, GDT>(), PB = PDT == 2 ? 4 : 2, GB = GDT == 2 ? 4 : 2, STEP = 8 * A8_BLOCK;  // elements from one of the warp's blocks to the next
+    A8Slot<PDT, GDT>* slots = reinterpret_cast<A8Slot<PDT, GDT>*>(a8_shared) + warp * STAGES;
     const long long i0 = b * A8_BLOCK + lane * 8;
     char* p_at = static_cast<char*>(t.p) + i0 * PB;
     const char* g_at = static_cast<const char*>(t.g) + i0 * GB;
@@ -308,7 +310,7 @@ __global__ void __launch_bounds__(256, PDT == 2 || GDT == 2 ? 2 : 3) adamw8_kern
       if (lane < 2) a8_copy<4>(lane ? &s.rs : &s.ms, (lane ? rs_at : ms_at) + ahead * 8);
     };
 #pragma unroll
-    for (int k = 0; k < A8_STAGES; ++k) {
+    for (int k = 0; k < STAGES; ++k) {
       if (k < iters) fetch(k, k);
       a8_copy_commit();
     }
@@ -316,7 +318,7 @@ __global__ void __launch_bounds__(256, PDT == 2 || GDT == 2 ? 2 : 3) adamw8_kern
     uint32_t e_hi = static_cast<uint32_t>(e >> 32), mix = mix_of(e);
     int stage = 0;
     for (int it = 0; it < iters; ++it) {
-      a8_copy_wait<A8_STAGES - 1>();
+      a8_copy_wait<STAGES - 1>();
       __syncwarp();
       const A8Slot<PDT, GDT>& s = slots[stage];
       uint64_t p[4], g[4];
@@ -325,7 +327,7 @@ __global__ void __launch_bounds__(256, PDT == 2 || GDT == 2 ? 2 : 3) adamw8_kern
       uint32_t mc[2] = {s.m[lane].x, s.m[lane].y}, rc[2] = {s.r[lane].x, s.r[lane].y};
       float ms = s.ms, rs = s.rs;
       __syncwarp();  // all lanes have read the scales
-      if (it + A8_STAGES < iters) fetch(A8_STAGES, stage);
+      if (it + STAGES < iters) fetch(STAGES, stage);
       a8_copy_commit();
       if (static_cast<uint32_t>(e >> 32) != e_hi) {
         e_hi = static_cast<uint32_t>(e >> 32);
@@ -341,7 +343,7 @@ __global__ void __launch_bounds__(256, PDT == 2 || GDT == 2 ? 2 : 3) adamw8_kern
       }
       p_at += STEP * PB; g_at += STEP * GB; m_at += STEP; r_at += STEP; ms_at += 8; rs_at += 8;
       e += STEP;
-      stage = stage + 1 < A8_STAGES ? stage + 1 : 0;
+      stage = stage + 1 < STAGES ? stage + 1 : 0;
     }
     b += 8LL * iters;
   }
@@ -442,9 +444,10 @@ extern "C" int msq_adamw8_multi(const unsigned long long* ptrs, const long long*
     const int n = count - at < MANY ? count - at : MANY;
     long long blocks = 0;
     for (int i = 0; i < n; ++i) blocks += (sizes[at + i] + A8_BLOCK - 1) / A8_BLOCK;
-    // A CTA's tile: long ones save the start-up of the copies (403M elements: 32 blocks 866 us, 128 blocks 831 us), short
-    // ones spread small lists over the SMs (one block per warp at the least).
-    const int tile_blocks = blocks >= 2 * 3 * 148 * 128 ? 128 : blocks >= 148 * 8 * 32 ? 32 : 8;
+    // A CTA's tile: long ones save the start-up of the copies (403M elements: 32 blocks 866 us, 128 blocks 831 us), but six
+    // tiles an SM keep the last wave short (6.3M fp32 elements: 8 blocks 26.4 us, 24 blocks 20.8 us, 56 blocks 22.6 us).
+    long long tile = blocks / (6 * 148) / 8 * 8;
+    const int tile_blocks = static_cast<int>(tile < 8 ? 8 : tile > 128 ? 128 : tile);
     int rc = -2;
 #define MSQ_A8(PD, GD)                                                                                      \
   rc = n <= FEW ? launch_adamw8<PD, GD, FEW>(ptrs + 6 * at, sizes + at, n, block0, tile_blocks, h, stream)            \
