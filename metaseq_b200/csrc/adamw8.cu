@@ -3,8 +3,8 @@
 // Blocks of 256 consecutive values of a tensor share one power-of-two scale per moment.  The first moment m is held as
 // e4m3 codes, the second as e4m3 codes of its root r = sqrt(v): r spans the range of |gradient|, v would need twice the
 // exponents.  One update of an element (fp32; the operations that make m and v are rounded one by one, so that the scales,
-// which come from comparing the largest of them with a power of two, do not depend on contraction; root and quotient use
-// the hardware's approximations, 2^-22):
+// which come from comparing the largest of them with a power of two, do not depend on contraction; the quotient uses the
+// hardware's reciprocal, 2^-22):
 //   g = grad * ctrl[0];  m = beta1 m + (1 - beta1) g;  v = beta2 r^2 + (1 - beta2) g^2;  r = sqrt(v)
 //   p = p - p * (lr * weight_decay);  p = p - (m / (r + eps)) * step_size
 // The parameter moves by the unrounded moments; then m and r are rounded for storage.
@@ -18,8 +18,8 @@
 //
 // One warp per block of 256: every lane takes eight values of p, g, m and r from a ring of asynchronous copies, the
 // block's largest magnitudes are found with two warp reductions, and everything is written in the same pass: 10 bytes a
-// parameter for 16-bit p and g.  What bounds it is instruction issue, about 50 per element (403M bf16 parameters: 0.82 ms,
-// 4.9 TB/s; the bytes alone would take 0.63 ms).
+// parameter for 16-bit p and g.  What bounds it is instruction issue, about 50 per element (403M bf16 parameters: 0.88 ms,
+// 4.6 TB/s; the bytes alone would take 0.63 ms.  With the hardware's root alone it is 0.82 ms, but one code in 2^18 is another).
 // The tensors' addresses travel in the kernel's parameters: no device table, no copy, nothing kept between calls.
 #include <cuda_fp8.h>
 
@@ -76,10 +76,26 @@ __device__ __forceinline__ float a8_max3(float a, float b, float c) {  // NaN if
   return r;
 }
 
-__device__ __forceinline__ float a8_sqrt(float x) {
+__device__ __forceinline__ float a8_rsqrt(float x) {
   float r;
-  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+__device__ __forceinline__ uint64_t a8_add_flush(uint64_t a, uint64_t b) {  // terms below the normal range (2^-150) count as zero
+  uint64_t r;
+  asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// Roots of two values >= 0: v * y with y = 1/sqrt(v) to 2^-22, and one Newton step on the residual, r - (r^2 - v) y / 2, whose
+// fused residual is exact.  That is off by 2^-44 before the last rounding, so the result is the rounded root but for one
+// value in a million next to a midpoint: a root off by more would draw other codes now and then.
+__device__ __forceinline__ uint64_t a8_root2(uint64_t v) {
+  float v0, v1;
+  f2_unpack(f2_add(v, f2_pack(1.17549435e-38f, 1.17549435e-38f)), v0, v1);  // keeps 0 * y finite, changes y by nothing above 2^-102
+  const uint64_t y = f2_pack(a8_rsqrt(v0), a8_rsqrt(v1));
+  const uint64_t r = f2_mul(v, y);
+  const uint64_t residual = f2_fma(r, r, f2_mul(v, f2_pack(-1.f, -1.f)));
+  return f2_fma(residual, f2_mul(y, f2_pack(-0.5f, -0.5f)), r);
 }
 __device__ __forceinline__ float a8_rcp(float x) {
   float r;
@@ -94,8 +110,12 @@ __device__ __forceinline__ int a8_root_scale_exp(uint32_t top_bits) {
   return top_bits < 0x00800000u ? -110 : (static_cast<int>(top_bits - 0x3F800000u + 0x3BFFFFu) >> 24) - 8;
 }
 
+// Gradients and roots are worked on times 2^12, v times 2^24 (exactly: powers of two): second moments down to fp32's smallest
+// then lie where the Newton step below has an exact residual (above 2^-103); gradients reach to 2^52.
+constexpr float A8_UP = 4096.f;
+
 struct Adam8Consts {
-  float gmul, beta1, omb1, beta2, omb2, eps, decay, step_size, minus_zero;
+  float gmul_up, beta1, omb1_down, beta2, omb2, eps_up, decay, step_size_up, minus_zero;
 };
 
 __device__ __forceinline__ float a8_lo(uint64_t v) { float a, b; f2_unpack(v, a, b); return a; }
@@ -112,26 +132,25 @@ __device__ __forceinline__ uint64_t a8_mul_rounded(uint64_t a, uint64_t b, float
 // and out, ms / rs: the block's scales in and out.  All lanes of the warp take part (two reductions).
 __device__ __forceinline__ void a8_update8(uint64_t (&p)[4], const uint64_t (&grad)[4], uint32_t (&mc)[2], uint32_t (&rc)[2],
                                            float& ms, float& rs, const Adam8Consts& c, uint32_t e0, uint32_t mix) {
-  uint64_t m[4], r[4];
+  uint64_t m[4], r[4], rr[4];
   float mmax = 0.f, vmax = 0.f;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int sh = (j & 1) * 16;
     const float2 mv = e4m3x2_to_float2(mc[j >> 1] >> sh), rv = e4m3x2_to_float2(rc[j >> 1] >> sh);
-    const uint64_t g = f2_mul(grad[j], a8_two(c.gmul));
+    const uint64_t g = f2_mul(grad[j], a8_two(c.gmul_up));
     m[j] = f2_mul(f2_pack(mv.x, mv.y), a8_two(ms));
-    r[j] = f2_mul(f2_pack(rv.x, rv.y), a8_two(rs));
-    m[j] = f2_add(a8_mul_rounded(m[j], a8_two(c.beta1), c.minus_zero), a8_mul_rounded(g, a8_two(c.omb1), c.minus_zero));
-    const uint64_t v = f2_add(a8_mul_rounded(f2_mul(r[j], r[j]), a8_two(c.beta2), c.minus_zero),
+    r[j] = f2_mul(f2_pack(rv.x, rv.y), a8_two(rs * A8_UP));
+    m[j] = f2_add(a8_mul_rounded(m[j], a8_two(c.beta1), c.minus_zero), a8_mul_rounded(g, a8_two(c.omb1_down), c.minus_zero));
+    const uint64_t v = a8_add_flush(a8_mul_rounded(f2_mul(r[j], r[j]), a8_two(c.beta2), c.minus_zero),
                               a8_mul_rounded(f2_mul(g, g), a8_two(c.omb2), c.minus_zero));
-    const float v0 = a8_lo(v), v1 = a8_hi(v);
     mmax = a8_max3(mmax, fabsf(a8_lo(m[j])), fabsf(a8_hi(m[j])));
-    vmax = a8_max3(vmax, v0, v1);
-    r[j] = f2_pack(a8_sqrt(v0), a8_sqrt(v1));
-    const uint64_t d = f2_add(r[j], a8_two(c.eps));
+    vmax = a8_max3(vmax, a8_lo(v), a8_hi(v));
+    r[j] = a8_root2(v);
+    const uint64_t d = f2_add(r[j], a8_two(c.eps_up));
     const uint64_t q = f2_mul(m[j], f2_pack(a8_rcp(a8_lo(d)), a8_rcp(a8_hi(d))));
     p[j] = f2_fma(p[j], a8_two(-c.decay), p[j]);
-    p[j] = f2_fma(q, a8_two(-c.step_size), p[j]);
+    p[j] = f2_fma(q, a8_two(-c.step_size_up), p[j]);
   }
   uint32_t mtop = __reduce_max_sync(0xffffffffu, __float_as_uint(mmax));
   uint32_t vtop = __reduce_max_sync(0xffffffffu, __float_as_uint(vmax));
@@ -150,12 +169,27 @@ __device__ __forceinline__ void a8_update8(uint64_t (&p)[4], const uint64_t (&gr
     mtop = __reduce_max_sync(0xffffffffu, mtop);
     vtop = __reduce_max_sync(0xffffffffu, vtop);
   }
-  const int mk = a8_scale_exp(mtop), rk = finite ? a8_root_scale_exp(vtop) : a8_scale_exp(vtop);
+  const int mk = a8_scale_exp(mtop), rk = max((finite ? a8_root_scale_exp(vtop) : a8_scale_exp(vtop)) - 12, -110);
   ms = __uint_as_float(static_cast<uint32_t>(127 + mk) << 23);
   rs = __uint_as_float(static_cast<uint32_t>(127 + rk) << 23);
-  const uint64_t minv = a8_two(__uint_as_float(static_cast<uint32_t>(127 - mk) << 23));
-  const uint64_t rinv = a8_two(__uint_as_float(static_cast<uint32_t>(127 - rk) << 23));
-  const uint64_t down = a8_two(__uint_as_float(7u << 23));  // 2^-120
+  // Down to where the codes stand: one product with 2^(-k - 120); a scale above 2^6 (2^-6), whose factor fp32 does not have, takes
+  // two (the first is exact, so either way there is one rounding).
+  if (mk <= 6 && rk <= -6) {
+    const uint64_t fm = a8_two(__uint_as_float(static_cast<uint32_t>(7 - mk) << 23)), fr = a8_two(__uint_as_float(static_cast<uint32_t>(7 - 12 - rk) << 23));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      m[j] = f2_mul(m[j], fm);
+      rr[j] = f2_mul(r[j], fr);
+    }
+  } else {
+    const uint64_t fm = a8_two(__uint_as_float(static_cast<uint32_t>(127 - mk) << 23)), fr = a8_two(__uint_as_float(static_cast<uint32_t>(127 - 12 - rk) << 23));
+    const uint64_t down = a8_two(__uint_as_float(7u << 23));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      m[j] = f2_mul(f2_mul(m[j], fm), down);
+      rr[j] = f2_mul(f2_mul(r[j], fr), down);
+    }
+  }
   // hash32((e0 + k) ^ mix) for k = 0 .. 7: e0 is a multiple of eight, so the first step's shift does not depend on k
   const uint32_t seed = e0 ^ mix, start = seed ^ (seed >> 16);
 #pragma unroll
@@ -163,15 +197,14 @@ __device__ __forceinline__ void a8_update8(uint64_t (&p)[4], const uint64_t (&gr
     uint32_t cm[4], cr[4], sg[4];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const uint64_t mm = f2_mul(f2_mul(m[2 * h + j], minv), down), rr = f2_mul(f2_mul(r[2 * h + j], rinv), down);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         uint32_t x = (start ^ static_cast<uint32_t>(4 * h + 2 * j + u)) * 0x7feb352dU;
         x = (x ^ (x >> 15)) * 0x846ca68bU;
         x ^= x >> 16;
-        sg[2 * j + u] = __float_as_uint(u ? a8_hi(mm) : a8_lo(mm));
+        sg[2 * j + u] = __float_as_uint(u ? a8_hi(m[2 * h + j]) : a8_lo(m[2 * h + j]));
         cm[2 * j + u] = a8_code_top(sg[2 * j + u], x & 0xFFFFu);
-        cr[2 * j + u] = a8_code_top(__float_as_uint(u ? a8_hi(rr) : a8_lo(rr)), x >> 16);
+        cr[2 * j + u] = a8_code_top(__float_as_uint(u ? a8_hi(rr[2 * h + j]) : a8_lo(rr[2 * h + j])), x >> 16);
       }
     }
     mc[h] = a8_top_bytes(cm[0], cm[1], cm[2], cm[3]) | (a8_top_bytes(sg[0], sg[1], sg[2], sg[3]) & 0x80808080u);
@@ -268,7 +301,8 @@ template <int PDT, int GDT, int COUNT>
 __global__ void __launch_bounds__(256, 3) adamw8_kernel(const __grid_constant__ Adam8Args<COUNT> a) {
   extern __shared__ uint4 a8_shared[];
   if (a.ctrl && a.ctrl[1] != 0.f) return;  // overflow: parameters and moments stay as they are
-  const Adam8Consts c{a.ctrl ? a.ctrl[0] : 1.f, a.beta1, a.omb1, a.beta2, a.omb2, a.eps, a.decay, a.step_size, a.minus_zero};
+  const Adam8Consts c{(a.ctrl ? a.ctrl[0] : 1.f) * A8_UP, a.beta1, a.omb1 * (1.f / A8_UP), a.beta2, a.omb2, a.eps * A8_UP, a.decay, a.step_size * A8_UP,
+                      a.minus_zero};
   int lo = 0, hi = a.count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;

@@ -1399,9 +1399,9 @@ def adamw8_step_multi(items, *, lr, beta1, beta2, eps, weight_decay, step, seed,
 
     The parameter moves by the moments in fp32.  They are then rounded to one of the two neighbouring codes, up with the
     probability of the remainder, by a draw from ``seed`` (a non-negative 64-bit number; pass another one every step)
-    and the element's number in the list, so equal calls give equal bits.  Values that are not finite are stored as
-    NaN.  ``ctrl`` is the device control block of ``clip_decision``: gradients are multiplied by ``ctrl[0]`` and nothing
-    changes when ``ctrl[1] != 0``."""
+    and the element's number in the list, so equal calls give equal bits.  Values that are not finite (gradients
+    beyond 2^52 among them) are stored as NaN.  ``ctrl`` is the device control block of ``clip_decision``: gradients are
+    multiplied by ``ctrl[0]`` and nothing changes when ``ctrl[1] != 0``."""
     items = list(items)
     if not items:
         return
@@ -1442,8 +1442,10 @@ def adamw8_step_multi(items, *, lr, beta1, beta2, eps, weight_decay, step, seed,
         g32 = whole(g) * gmul
         m = whole(mc) * ms[:, None] * beta1 + g32 * omb1
         r = whole(rc) * rs[:, None]
-        r = (r * r) * beta2 + (g32 * g32) * omb2
-        r = torch.sqrt(torch.where(r < 2.0 ** -126, torch.zeros_like(r), r))  # below fp32's normal range: zero
+        # v times 2^24, as in the kernel: its terms then lie in fp32's normal range
+        up = 2.0 ** 12
+        v = (r * up) * (r * up) * beta2 + (g32 * up) * (g32 * up) * omb2
+        r = torch.sqrt(torch.where(torch.isinf(v), torch.full_like(v, float("nan")), v)) / up
         q = whole(p)
         q = q - q * decay
         q = q - (m / (r + eps)) * step_size
