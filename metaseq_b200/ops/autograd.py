@@ -289,10 +289,11 @@ class EmbeddingFn(torch.autograd.Function):
                 return F.embed_grad_sorted(index, dy, rows, factor, pad_idx, start, out=out, accumulate=acc)
             return _direct_grad(param, compute)
 
+        tokens = tokens.long()
         dt = table_grad(tokens, nt, scale, vstart, tok_w)
         dp = None
         if pos_w is not None:  # without position numbers nothing was looked up
-            index = positions if positions is not None else torch.full_like(tokens, pad_idx)
+            index = positions.reshape(tokens.shape).long() if positions is not None else torch.full_like(tokens, pad_idx)
             dp = table_grad(index, np_, 1.0, 0, pos_w)
         return None, None, dt, dp, None, None, None
 

@@ -676,8 +676,8 @@ def embed_grad_sorted(tokens, dy, rows: int, scale: float = 1.0, pad_idx: int = 
     if dy.dim() < 1 or dy.shape[:-1] != tokens.shape:
         raise ValueError(f"embed_grad_sorted: dy {tuple(dy.shape)} does not extend tokens {tuple(tokens.shape)}")
     D = dy.shape[-1]
-    if rows <= 0 or D <= 0:
-        raise ValueError(f"embed_grad_sorted: the table has no elements (rows={rows}, D={D})")
+    if rows <= 0 or D <= 0 or rows >= 1 << 31:
+        raise ValueError(f"embed_grad_sorted: the table has no elements, or 2^31 rows and more (rows={rows}, D={D})")
     if out is None:
         if accumulate:
             raise ValueError("embed_grad_sorted: accumulate needs the table to add to (out)")
@@ -972,7 +972,7 @@ def _linear_ce_check(x, weight, target):
 
 def _linear_ce_kernel_ok(x2, weight) -> bool:
     n, D = x2.shape
-    return (use_kernels(x2) and n > 0 and D % 8 == 0 and n <= 1 << 24 and weight.shape[0] <= 1 << 24
+    return (use_kernels(x2) and n > 0 and D % 8 == 0 and D <= 1 << 20 and n <= 1 << 24 and weight.shape[0] <= 1 << 24
             and weight.stride(1) == 1 and weight.stride(0) % 8 == 0 and weight.stride(0) >= D and weight.data_ptr() % 16 == 0)
 
 
@@ -1411,7 +1411,10 @@ def adamw8_step_multi(items, *, lr, beta1, beta2, eps, weight_decay, step, seed,
     sizes = _adamw8_check(flat)
     if step < 1:
         raise ValueError(f"adamw8_step_multi: the first step is 1, not {step}")
-    seed = int(seed)
+    addresses = set(map(torch.Tensor.data_ptr, flat[0::6]))
+    if len(addresses) != len(items) and len(addresses) - (0 in addresses) != len([k for k in sizes if k]):
+        raise ValueError("adamw8_step_multi: a parameter stands in the list twice")
+    lr, beta1, beta2, eps, weight_decay, seed = float(lr), float(beta1), float(beta2), float(eps), float(weight_decay), int(seed)
     if not 0 <= seed < 1 << 64:
         raise ValueError("adamw8_step_multi: seed must be in [0, 2^64)")
     p0, g0 = flat[0], flat[1]

@@ -195,6 +195,10 @@ def test_refusals():
                       ((p, g.to("meta"), m, ms, r, rs), "different devices")]:
         with pytest.raises(ValueError, match=text):
             step(*bad)
+    with pytest.raises(ValueError, match="twice"):
+        F.adamw8_step_multi([ok, ok], **HYPER, step=1, seed=0)
+    empty = _items([0, 0, 5], torch.float32, torch.float32, "cpu", 1)
+    F.adamw8_step_multi(empty, **HYPER, step=1, seed=0)  # tensors without elements share an address
     with pytest.raises(ValueError, match="first step"):
         step(*ok, step=0)
     with pytest.raises(ValueError, match="seed"):

@@ -121,6 +121,18 @@ def test_refusals():
         F.embed_grad_sorted(tokens, dy, 0)
     with pytest.raises(ValueError, match="different devices"):
         F.embed_grad_sorted(tokens, dy.to("meta"), 3)
+    with pytest.raises(ValueError, match=r"2\^31"):
+        F.embed_grad_sorted(tokens, dy, 1 << 31)
+
+
+def test_embedding_backward_takes_other_shapes_of_positions():
+    """Positions given flat, and 32-bit tokens on the CPU, as the lookup takes them."""
+    w = torch.randn(9, 8).requires_grad_()
+    p = torch.randn(12, 8).requires_grad_()
+    tokens, positions = torch.randint(0, 9, (2, 6)), torch.arange(12)
+    ag.embedding(tokens.int(), positions, w, p, 1.0, -1).sum().backward()
+    assert torch.equal(p.grad, torch.ones_like(p))
+    assert torch.equal(w.grad[:, 0], torch.bincount(tokens.reshape(-1), minlength=9).float())
 
 
 @pytest.mark.parametrize("device", DEVICES)
