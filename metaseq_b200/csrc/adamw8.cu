@@ -66,7 +66,7 @@ __device__ __forceinline__ int a8_scale_exp(uint32_t top_bits) {
 // codes below 2^-6, multiples of 2^-9, as fp32 denormals (these products do not flush them).  The bits underneath are the
 // remainder; adding 16 random bits on top of them rounds up with its probability, for both kinds alike.  The sum is formed
 // four bits higher (multiply-adds: the ALU pipe is what bounds this kernel), so that the code is the top byte.
-__device__ __forceinline__ uint32_t a8_code_top(uint32_t bits, uint32_t rnd) { return bits * 16u + rnd * 256u; }
+__device__ __forceinline__ uint32_t a8_code_top(uint32_t bits, uint32_t rnd_256) { return bits * 16u + rnd_256; }
 __device__ __forceinline__ uint32_t a8_top_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
 }
@@ -201,10 +201,11 @@ __device__ __forceinline__ void a8_update8(uint64_t (&p)[4], const uint64_t (&gr
       for (int u = 0; u < 2; ++u) {
         uint32_t x = (start ^ static_cast<uint32_t>(4 * h + 2 * j + u)) * 0x7feb352dU;
         x = (x ^ (x >> 15)) * 0x846ca68bU;
-        x ^= x >> 16;
+        // the last step, x ^ (x >> 16), and its halves times 256: the upper half is left as it is
+        const uint32_t high = __byte_perm(x, 0u, 0x4324), low = __byte_perm(x, 0u, 0x4104) ^ high;
         sg[2 * j + u] = __float_as_uint(u ? a8_hi(m[2 * h + j]) : a8_lo(m[2 * h + j]));
-        cm[2 * j + u] = a8_code_top(sg[2 * j + u], x & 0xFFFFu);
-        cr[2 * j + u] = a8_code_top(__float_as_uint(u ? a8_hi(rr[2 * h + j]) : a8_lo(rr[2 * h + j])), x >> 16);
+        cm[2 * j + u] = a8_code_top(sg[2 * j + u], low);
+        cr[2 * j + u] = a8_code_top(__float_as_uint(u ? a8_hi(rr[2 * h + j]) : a8_lo(rr[2 * h + j])), high);
       }
     }
     mc[h] = a8_top_bytes(cm[0], cm[1], cm[2], cm[3]) | (a8_top_bytes(sg[0], sg[1], sg[2], sg[3]) & 0x80808080u);
