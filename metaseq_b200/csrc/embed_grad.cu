@@ -4,7 +4,7 @@
 // bits.  Tokens equal to pad_idx or outside [vocab_start, vocab_start + table rows) contribute nothing.
 //
 // What bounds it is memory: every kept row of dy is read once, and either the whole table is written once (new table) or
-// the touched rows are read and written (accumulate).  Up to 1024 tokens one kernel does everything (after a zero fill of a
+// the touched rows are read and written (accumulate).  Up to 256 tokens one kernel does everything (after a zero fill of a
 // new table): every CTA sorts all tokens in shared memory and sums 256 columns.  Above that, three launches:
 //   1. one cluster of eight CTAs sorts (token, row) pairs by a stable radix sort while the other CTAs, when the table is
 //      new, fill its first rows with zeros;
@@ -307,17 +307,9 @@ struct Vec8 {
   }
 };
 
-// out[elem .. elem + 7] = (accumulate ? itself : 0) + scale * f, rounded once
+// out[elem .. elem + 7] = o + scale * f, rounded once; o: what is added to
 template <int DT>
-__device__ __forceinline__ void store_row8(void* out, long long elem, const float (&f)[8], float scale, int accumulate) {
-  float o[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) o[j] = 0.f;
-  if (accumulate) {
-    Vec8<DT> old;
-    old.load(out, elem);
-    old.add_to(o);
-  }
+__device__ __forceinline__ void store_sum8(void* out, long long elem, const float (&f)[8], float scale, float (&o)[8]) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) o[j] = fmaf(f[j], scale, o[j]);
   if constexpr (DT == 2) {
@@ -329,6 +321,83 @@ __device__ __forceinline__ void store_row8(void* out, long long elem, const floa
         make_uint4(pack2<DT == 1>(o[0], o[1]), pack2<DT == 1>(o[2], o[3]), pack2<DT == 1>(o[4], o[5]), pack2<DT == 1>(o[6], o[7]));
   }
 }
+template <int DT>
+__device__ __forceinline__ void store_row8(void* out, long long elem, const float (&f)[8], float scale, int accumulate) {
+  float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (accumulate) {
+    Vec8<DT> old;
+    old.load(out, elem);
+    old.add_to(o);
+  }
+  store_sum8<DT>(out, elem, f, scale, o);
+}
+
+// Sums the runs of equal tokens in `count` consecutive sorted pairs; the tokens before and behind them tell which runs
+// cross.  Runs inside are written; the first and the last, where they cross, are handed to head(f) and tail(f) by finish().
+// Rows are requested a batch at a time, with the old rows that the batch's finished runs are added to (one after the other,
+// a read of the table behind every run, 16 runs of one token each took 20 us).
+template <int DT, bool ACC>
+struct RunWalker {
+  static constexpr int BATCH = DT == 2 && !ACC ? 8 : 4;  // 16 bits: eight rows 94 us instead of 74 (16384 x 2048); fp32: four 41 us instead of 26 (6007 x 1000)
+  const void* dy;
+  long long ldy;
+  void* out;
+  long long ldo;
+  float scale;
+  uint32_t none, prev;
+  int col;
+  bool live;
+  float f[8];
+  bool first;  // no run has ended yet
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = 0.f;
+  }
+  template <typename Key, typename Row, typename Head>
+  __device__ __forceinline__ void walk(int count, Key key_of, Row row_of, uint32_t behind, Head head) {
+    for (int e0 = 0; e0 < count; e0 += BATCH) {
+      Vec8<DT> v[BATCH], old[ACC ? BATCH : 1];
+      uint32_t key[BATCH + 1];
+#pragma unroll
+      for (int e = 0; e <= BATCH; ++e) key[e] = e0 + e < count ? key_of(e0 + e) : behind;
+#pragma unroll
+      for (int e = 0; e < BATCH; ++e) {
+        const uint32_t row = row_of(e0 + e);
+        if (e0 + e >= count || key[e] == none || !live) continue;
+        v[e].load(dy, static_cast<long long>(row) * ldy + col);
+        if constexpr (ACC) {
+          if (key[e] != key[e + 1]) old[e].load(out, static_cast<long long>(key[e]) * ldo + col);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < BATCH; ++e) {
+        if (e0 + e >= count) break;
+        if (key[e] != none && live) v[e].add_to(f);
+        if (key[e] != key[e + 1]) {
+          if (key[e] != none) {
+            if (first && key[e] == prev) {
+              head(f);
+            } else if (live) {
+              float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+              if constexpr (ACC) old[e].add_to(o);
+              store_sum8<DT>(out, static_cast<long long>(key[e]) * ldo + col, f, scale, o);
+            }
+          }
+          clear();
+          first = false;
+        }
+      }
+    }
+  }
+  // after the last pair, with its token and the one behind it
+  template <typename Head, typename Tail>
+  __device__ __forceinline__ void finish(uint32_t last, uint32_t behind, Head head, Tail tail) {
+    if (last == none || last != behind) return;
+    if (first && last == prev) head(f);
+    else tail(f);
+  }
+};
 
 struct EmbedGradSum {
   const uint2* pairs;
@@ -376,9 +445,8 @@ __device__ void embed_grad_fill(const EmbedGradSum& s) {
   }
 }
 
-// One warp: `chunk` sorted pairs, 256 columns (eight per lane).  Rows are requested eight at a time so that a warp keeps
-// 4 KB of reads in flight.
-template <int DT>
+// One warp: `chunk` sorted pairs, 256 columns (eight per lane).
+template <int DT, bool ACC>
 __global__ void __launch_bounds__(256) embed_grad_sum_kernel(const EmbedGradSum s) {
   dependents_launch();
   dependents_wait();
@@ -390,60 +458,32 @@ __global__ void __launch_bounds__(256) embed_grad_sum_kernel(const EmbedGradSum 
   const int lane = threadIdx.x & 31;
   const int c = static_cast<int>(wid / s.slices);
   if (c >= s.chunks) return;
-  const int col = static_cast<int>(wid - static_cast<long long>(c) * s.slices) * 256 + lane * 8;
-  const bool live = col < s.D;
   const uint32_t none = static_cast<uint32_t>(s.rows);
   const int p0 = c * s.chunk, p1 = min(p0 + s.chunk, s.n);
-  const uint32_t prev = p0 > 0 ? s.pairs[p0 - 1].x : none;
-  const uint32_t next = p1 < s.n ? s.pairs[p1].x : none;
-  float f[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = 0.f;
-  uint32_t run = none;
-  bool first = true;  // no run of this chunk has ended yet
-
-  auto flush = [&](bool at_end) {
-    if (run == none || !live) return;
-    const bool from_before = first && run == prev;
-    const bool goes_on = at_end && run == next;
-    if (from_before || goes_on) {
-      float4* dst = reinterpret_cast<float4*>((from_before ? s.head : s.tail) + static_cast<long long>(c) * s.D + col);
-      dst[0] = make_float4(f[0], f[1], f[2], f[3]);
-      dst[1] = make_float4(f[4], f[5], f[6], f[7]);
-    } else {
-      store_row8<DT>(s.out, static_cast<long long>(run) * s.ldo + col, f, s.scale, s.accumulate);
-    }
+  RunWalker<DT, ACC> w;
+  w.dy = s.dy; w.ldy = s.ldy; w.out = s.out; w.ldo = s.ldo; w.scale = s.scale;
+  w.none = none;
+  w.col = static_cast<int>(wid - static_cast<long long>(c) * s.slices) * 256 + lane * 8;
+  w.live = w.col < s.D;
+  w.prev = p0 > 0 ? s.pairs[p0 - 1].x : none;
+  w.first = true;
+  w.clear();
+  auto keep = [&](float* to, const float (&f)[8]) {
+    if (!w.live) return;
+    float4* dst = reinterpret_cast<float4*>(to + static_cast<long long>(c) * s.D + w.col);
+    dst[0] = make_float4(f[0], f[1], f[2], f[3]);
+    dst[1] = make_float4(f[4], f[5], f[6], f[7]);
   };
-
+  auto head = [&](const float (&f)[8]) { keep(s.head, f); };
+  uint32_t last = none, behind = none;
   for (int q0 = p0; q0 < p1; q0 += 32) {
     const uint2 mine = q0 + lane < p1 ? s.pairs[q0 + lane] : make_uint2(none, 0u);
     const int cnt = min(32, p1 - q0);
-    for (int e0 = 0; e0 < cnt; e0 += 8) {
-      Vec8<DT> v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t key = __shfl_sync(0xffffffffu, mine.x, e0 + e);
-        const uint32_t row = __shfl_sync(0xffffffffu, mine.y, e0 + e);
-        if (key != none && live) v[e].load(s.dy, static_cast<long long>(row) * s.ldy + col);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t key = __shfl_sync(0xffffffffu, mine.x, e0 + e);
-        if (e0 + e >= cnt) break;
-        if (e0 + e > 0 || q0 > p0) {
-          if (key != run) {
-            flush(false);
-            first = false;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = 0.f;
-          }
-        }
-        run = key;
-        if (key != none && live) v[e].add_to(f);
-      }
-    }
+    behind = q0 + cnt < s.n ? s.pairs[q0 + cnt].x : none;
+    w.walk(cnt, [&](int i) { return __shfl_sync(0xffffffffu, mine.x, i); }, [&](int i) { return __shfl_sync(0xffffffffu, mine.y, i & 31); }, behind, head);
+    last = __shfl_sync(0xffffffffu, mine.x, cnt - 1);
   }
-  flush(true);
+  w.finish(last, behind, head, [&](const float (&f)[8]) { keep(s.tail, f); });
 }
 
 // Runs that begin in chunk c and cross its border: tail[c] + head[c + 1] + ... in ascending order, 256 columns per warp.  A
@@ -530,9 +570,11 @@ __global__ void __launch_bounds__(256) embed_grad_join_kernel(const EmbedGradSum
   }
 }
 
-// Few tokens: a CTA per 256 columns finds every token's place by counting (equal tokens keep their order), its 32 warps sum
+// Few tokens: a CTA per 256 columns finds every token's place by counting (equal tokens keep their order), its 16 warps sum
 // contiguous parts of the sorted list, and runs that cross from one warp to the next are joined through shared memory.
-constexpr int EG_FEW = 1024;
+constexpr int EG_FEW = 256;  // tokens.  768 columns: 128 tokens 5.8 us (three launches 14.1), 256 11.1 (14.5), 400 20.1 (14.8)
+constexpr int EG_FEW_THREADS = 512;
+constexpr int EG_FEW_WARPS = EG_FEW_THREADS / 32;
 
 struct EmbedGradFew {
   const long long* tokens;
@@ -545,14 +587,11 @@ struct EmbedGradFew {
   float scale;
 };
 
-template <int DT>
-__global__ void __launch_bounds__(1024, 1) embed_grad_few_kernel(const EmbedGradFew s) {
-  extern __shared__ float few_smem[];
-  float* head = few_smem;               // [32][256]
-  float* tail = head + 32 * 256;        // [32][256]
-  uint32_t* keys = reinterpret_cast<uint32_t*>(tail + 32 * 256);  // [EG_FEW], padded with the largest number
-  uint32_t* skey = keys + EG_FEW;       // sorted
-  uint32_t* srow = skey + EG_FEW;
+template <int DT, bool ACC>
+__global__ void __launch_bounds__(EG_FEW_THREADS, 1) embed_grad_few_kernel(const EmbedGradFew s) {
+  __shared__ float head_s[EG_FEW_WARPS][8][32], tail_s[EG_FEW_WARPS][8][32];
+  __shared__ __align__(16) uint32_t keys[EG_FEW];  // padded with the largest number
+  __shared__ uint32_t skey[EG_FEW], srow[EG_FEW];   // sorted
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t none = static_cast<uint32_t>(s.rows);
   dependents_wait();
@@ -562,7 +601,7 @@ __global__ void __launch_bounds__(1024, 1) embed_grad_few_kernel(const EmbedGrad
     const bool in = t != s.pad_idx && t >= s.vocab_start && t < s.vocab_start + s.rows;
     mine = in ? static_cast<uint32_t>(t - s.vocab_start) : none;
   }
-  keys[tid] = mine;
+  if (tid < EG_FEW) keys[tid] = mine;
   __syncthreads();
   if (warp * 32 < s.n) {
     int rank = 0;
@@ -578,60 +617,38 @@ __global__ void __launch_bounds__(1024, 1) embed_grad_few_kernel(const EmbedGrad
     }
   }
   __syncthreads();
-  const int per = (s.n + 31) >> 5;
+  const int per = (s.n + EG_FEW_WARPS - 1) / EG_FEW_WARPS;
   const int p0 = min(warp * per, s.n), p1 = min(p0 + per, s.n);
-  const int col = blockIdx.x * 256 + lane * 8;
-  const bool live = col < s.D;
-  const uint32_t prev = p0 > 0 ? skey[p0 - 1] : none, next = p1 < s.n ? skey[p1] : none;
-  float f[8];
+  RunWalker<DT, ACC> w;
+  w.dy = s.dy; w.ldy = s.ldy; w.out = s.out; w.ldo = s.ldo; w.scale = s.scale;
+  w.none = none;
+  w.col = blockIdx.x * 256 + lane * 8;
+  w.live = w.col < s.D;
+  w.prev = p0 > 0 ? skey[p0 - 1] : none;
+  w.first = true;
+  w.clear();
+  auto head = [&](const float (&f)[8]) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = 0.f;
-  uint32_t run = none;
-  bool first = true;
-  auto keep = [&](float* to) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) to[warp * 256 + j * 32 + lane] = f[j];
+    for (int j = 0; j < 8; ++j) head_s[warp][j][lane] = f[j];
   };
-  auto flush = [&](bool at_end) {
-    if (run == none) return;
-    if (first && run == prev) keep(head);
-    else if (at_end && run == next) keep(tail);
-    else if (live) store_row8<DT>(s.out, static_cast<long long>(run) * s.ldo + col, f, s.scale, s.accumulate);
+  auto tail = [&](const float (&f)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) tail_s[warp][j][lane] = f[j];
   };
-  for (int q0 = p0; q0 < p1; q0 += 8) {
-    Vec8<DT> v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (q0 + e < p1 && skey[q0 + e] != none && live) v[e].load(s.dy, static_cast<long long>(srow[q0 + e]) * s.ldy + col);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (q0 + e >= p1) break;
-      const uint32_t key = skey[q0 + e];
-      if (q0 + e > p0 && key != run) {
-        flush(false);
-        first = false;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = 0.f;
-      }
-      run = key;
-      if (key != none && live) v[e].add_to(f);
-    }
-  }
-  flush(true);
+  const uint32_t last = p1 > p0 ? skey[p1 - 1] : none, behind = p1 < s.n ? skey[p1] : none;
+  w.walk(p1 - p0, [&](int i) { return skey[p0 + i]; }, [&](int i) { return srow[min(p0 + i, EG_FEW - 1)]; }, behind, head);
+  w.finish(last, behind, head, tail);
   __syncthreads();
   // the warp in whose part a crossing run begins adds the parts that follow
-  if (p1 > p0 && p1 < s.n) {
-    const uint32_t key = skey[p1 - 1];
-    const bool began_here = !(skey[p0] == key && prev == key);
-    if (key != none && next == key && began_here) {
+  if (last != none && behind == last && !(skey[p0] == last && w.prev == last)) {
+    float f[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = tail[warp * 256 + j * 32 + lane];
-      for (int w = warp + 1; w < 32 && w * per < s.n && skey[w * per] == key; ++w) {
+    for (int j = 0; j < 8; ++j) f[j] = tail_s[warp][j][lane];
+    for (int q = warp + 1; q < EG_FEW_WARPS && q * per < s.n && skey[q * per] == last; ++q) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] += head[w * 256 + j * 32 + lane];
-      }
-      if (live) store_row8<DT>(s.out, static_cast<long long>(key) * s.ldo + col, f, s.scale, s.accumulate);
+      for (int j = 0; j < 8; ++j) f[j] += head_s[q][j][lane];
     }
+    if (w.live) store_row8<DT>(s.out, static_cast<long long>(last) * s.ldo + w.col, f, s.scale, ACC);
   }
 }
 
@@ -659,25 +676,23 @@ static cudaError_t eg_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, si
 
 template <int DT>
 static cudaError_t eg_launch_few(const EmbedGradFew& f, cudaStream_t stream) {
-  constexpr int smem = 2 * 32 * 256 * 4 + 3 * EG_FEW * 4;
-  const cudaError_t err = cudaFuncSetAttribute(embed_grad_few_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (err != cudaSuccess) return err;
   const dim3 grid((f.D + 255) / 256);
-  if (!f.accumulate) return eg_launch(embed_grad_few_kernel<DT>, grid, dim3(1024), smem, stream, f);  // behind the fill
-  embed_grad_few_kernel<DT><<<grid, 1024, smem, stream>>>(f);
+  if (!f.accumulate) return eg_launch(embed_grad_few_kernel<DT, false>, grid, dim3(EG_FEW_THREADS), 0, stream, f);  // behind the fill
+  embed_grad_few_kernel<DT, true><<<grid, EG_FEW_THREADS, 0, stream>>>(f);
   return cudaGetLastError();
 }
 
 template <int DT>
 static cudaError_t eg_launch_sums(const EmbedGradSum& su, unsigned blocks, dim3 join, cudaStream_t stream) {
-  const cudaError_t err = eg_launch(embed_grad_sum_kernel<DT>, dim3(blocks), dim3(256), 0, stream, su);
+  const cudaError_t err = eg_launch(su.accumulate ? embed_grad_sum_kernel<DT, true> : embed_grad_sum_kernel<DT, false>, dim3(blocks), dim3(256), 0, stream, su);
   return err != cudaSuccess ? err : eg_launch(embed_grad_join_kernel<DT>, join, dim3(256), 0, stream, su);
 }
 
+// Pairs a warp: as few as keep the SMs busy with one wave of warps or so (16384 x 2048: 8 pairs 79.4 us, 16 74.1, 32 72.5).
 static int eg_chunk(long long n, int D) {
   const long long slices = (D + 255) / 256;
   int chunk = 8;
-  while (chunk < 256 && n * slices > 2LL * chunk * 4736) chunk *= 2;
+  while (chunk < 256 && n * slices > chunk * 4736LL) chunk *= 2;
   return chunk;
 }
 

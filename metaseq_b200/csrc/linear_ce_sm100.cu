@@ -38,7 +38,6 @@ constexpr uint32_t LC_EPI_BYTES = LC_EPI_WARPS * 4096;  // per warp: 32 rows x 1
 constexpr uint32_t LC_SMEM = LC_STAGES * (LC_A_BYTES + LC_B_BYTES) + LC_EPI_BYTES + 1024 + 256;
 constexpr uint32_t LC_TMEM_COLS = 2 * LC_BN;
 constexpr float LC_LOG2E = 1.4426950408889634f;
-constexpr float LC_LN2 = 0.6931471805599453f;
 
 struct LceParams {
   int M, N, K;
@@ -597,9 +596,10 @@ __global__ void __launch_bounds__(1024) lce_merge_kernel(const LceMerge s) {
   float loss = 0.f;
   if (lane == 0) {
     if (mine < count) {
-      const float l2 = log2f(sum);
-      s.lse2[mine] = fmaf(mx, LC_LOG2E, l2);
-      loss = mx - s.st_tgt[mine] + l2 * LC_LN2;
+      // in 64 bits: the loss of a confident token is a small difference, and the hardware's logarithm next to 1 is off by 2^-22
+      const double ln = log(static_cast<double>(sum));
+      s.lse2[mine] = static_cast<float>((static_cast<double>(mx) + ln) * 1.4426950408889634);
+      loss = static_cast<float>(static_cast<double>(mx) - static_cast<double>(s.st_tgt[mine]) + ln);
       s.loss[s.rows[mine]] = loss;
     } else if (mine < ((s.n + 255) & ~255)) {
       s.lse2[mine] = INFINITY;
