@@ -58,13 +58,10 @@ class _Counted:
 class _CountingLib:
     def __init__(self, lib):
         self._lib = lib
-        self._cache = {}
 
-    def __getattr__(self, name):
-        c = self._cache.get(name)
-        if c is None:
-            c = _Counted(getattr(self._lib, name), _KERNELS_PER_CALL.get(name, 1))
-            self._cache[name] = c
+    def __getattr__(self, name):  # reached once per entry point: the wrapper then is an attribute of its own
+        c = _Counted(getattr(self._lib, name), _KERNELS_PER_CALL.get(name, 1))
+        setattr(self, name, c)
         return c
 
 

@@ -673,22 +673,22 @@ def embed_grad_sorted(tokens, dy, rows: int, scale: float = 1.0, pad_idx: int = 
     order, and rounded once, so equal inputs give equal bits (``embed_bwd`` adds with atomics, in any order)."""
     if tokens.dtype != torch.int64:
         raise ValueError(f"embed_grad_sorted: tokens must be int64, not {tokens.dtype}")
-    if dy.dim() < 1 or dy.shape[:-1] != tokens.shape:
+    if dy.dim() != tokens.dim() + 1 or dy.shape[:-1] != tokens.shape:
         raise ValueError(f"embed_grad_sorted: dy {tuple(dy.shape)} does not extend tokens {tuple(tokens.shape)}")
     D = dy.shape[-1]
+    n = tokens.numel()
     if rows <= 0 or D <= 0 or rows >= 1 << 31:
         raise ValueError(f"embed_grad_sorted: the table has no elements, or 2^31 rows and more (rows={rows}, D={D})")
     if out is None:
         if accumulate:
             raise ValueError("embed_grad_sorted: accumulate needs the table to add to (out)")
-    elif tuple(out.shape) != (rows, D):
+    elif out.shape != (rows, D):
         raise ValueError(f"embed_grad_sorted: out is {tuple(out.shape)}, the table is {(rows, D)}")
     _same_device("embed_grad_sorted", tokens, dy, out)
-    tok = tokens.reshape(-1).contiguous()
-    dy2 = dy.reshape(-1, D)
+    tok, dy2 = (tokens, dy) if dy.dim() == 2 else (tokens.reshape(-1), dy.reshape(-1, D))
+    tok = tok.contiguous()
     if dy2.stride(1) != 1 or dy2.stride(0) % 8 or dy2.data_ptr() % 16:
         dy2 = dy2.contiguous()
-    n = tok.numel()
     if _float_kernels(dy2) and D % 8 == 0 and dy2.data_ptr() % 16 == 0 and n <= 1 << 30 and (
             out is None or (out.dtype == dy2.dtype and out.stride(1) == 1 and out.stride(0) % 8 == 0
                             and (rows == 1 or out.stride(0) >= D) and out.data_ptr() % 16 == 0
@@ -699,10 +699,10 @@ def embed_grad_sorted(tokens, dy, rows: int, scale: float = 1.0, pad_idx: int = 
                 out = torch.empty((rows, D), dtype=dy2.dtype, device=dy2.device)
             size = lib.msq_embed_grad_workspace(n, D)
             ws = torch.empty(size, dtype=torch.uint8, device=dy2.device) if size else None
-            rc = lib.msq_embed_grad_sorted(_lib.ptr(tok), _lib.ptr(dy2), dy2.stride(0), _lib.ptr(out),
+            rc = lib.msq_embed_grad_sorted(tok.data_ptr(), dy2.data_ptr(), dy2.stride(0), out.data_ptr(),
                                            out.stride(0) if rows > 1 else D, n, rows, D, float(scale), int(vocab_start),
-                                           int(pad_idx), int(accumulate), _lib.dtype_code(dy2.dtype), _lib.ptr(ws),
-                                           _lib.stream_ptr())
+                                           int(pad_idx), int(accumulate), _lib.dtype_code(dy2.dtype),
+                                           ws.data_ptr() if size else None, _lib.stream_ptr())
         _lib.check_rc(rc, "msq_embed_grad_sorted")
         return out
     if dy2.is_cuda and dy2.dtype in (torch.float16, torch.bfloat16) and (out is None or out.dtype == dy2.dtype):

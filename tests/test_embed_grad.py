@@ -179,7 +179,7 @@ def test_equal_inputs_give_equal_bits_and_graph_replay():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("n,rows,D", [(70001, 50272, 128), (20000, 300000, 8), (3, 1 << 20, 8), (40000, 2, 2048)])
+@pytest.mark.parametrize("n,rows,D", [(70001, 50272, 128), (20000, 300000, 8), (3, 1 << 20, 8), (40000, 2, 2048), (3000, 5000011, 8), (9001, 50272, 72)])
 def test_large_batches_and_tables(n, rows, D):
     g = torch.Generator(device="cuda").manual_seed(n)
     tokens = torch.randint(0, rows, (n,), generator=g, device="cuda")

@@ -223,7 +223,7 @@ BASE = ["--task", "dummy_lm", "--dict-size", "124", "--tokens-per-sample", "16",
         "--warmup-updates", "1"]
 
 
-def _losses(save_dir, extra, updates=4):
+def _trainer(save_dir, extra):
     argv = BASE + ["--save-dir", str(save_dir), *extra]
     cfg = convert_namespace_to_config(options.parse_args_and_arch(options.get_training_parser(), input_args=argv))
     torch.manual_seed(1)
@@ -231,7 +231,11 @@ def _losses(save_dir, extra, updates=4):
     model, criterion = build_model_and_criterion(cfg, task)
     trainer = Trainer(cfg, task, model, criterion)
     task.load_dataset("train")
-    batch = task.dataset("train").collater([0, 1])
+    return trainer, task.dataset("train").collater([0, 1])
+
+
+def _losses(save_dir, extra, updates=4):
+    trainer, batch = _trainer(save_dir, extra)
     logs = [trainer.train_step([batch]) for _ in range(updates)]
     valid = trainer.valid_step(batch)
     return [float(log["loss"]) for log in logs if log is not None], float(valid["loss"]), trainer
@@ -259,6 +263,25 @@ def test_training_with_all_three(tmp_path, extra):
     assert len(losses) >= 4 and all(map(math.isfinite, losses)) and math.isfinite(valid)
     states = trainer.optimizer.optimizer.state.values()
     assert states and all("exp_avg_8" in s for s in states)
+
+
+@pytest.mark.parametrize("extra", [["--cpu"], ["--cpu", "--memory-efficient-fp16", "--fp16-init-scale", "4"], ["--cpu", "--fp16",
+                                   "--fp16-init-scale", "4"],
+                                   pytest.param(["--memory-efficient-fp16", "--fp16-init-scale", "4"], marks=pytest.mark.gpu)])
+def test_checkpointed_run_resumes_with_eight_bit_moments(tmp_path, extra):
+    flags = extra + ["--criterion", "cross_entropy", "--logits-free", "--fp8-adam-stats"]
+    trainer, batch = _trainer(tmp_path, flags)
+    for _ in range(3):
+        trainer.train_step([batch])
+    path = str(tmp_path / "resume.pt")
+    trainer.save_checkpoint(path, {"train_iterator": {"epoch": 1}})
+    want = [float(trainer.train_step([batch])["loss"]) for _ in range(3)]
+    other, batch = _trainer(tmp_path / "b", flags)
+    other.load_checkpoint(path)
+    states = list(other.optimizer.optimizer.state.values())
+    assert states and all(s["exp_avg_8"].dtype == torch.float8_e4m3fn for s in states)
+    got = [float(other.train_step([batch])["loss"]) for _ in range(3)]
+    assert got == want
 
 
 def test_logits_free_needs_the_whole_vocabulary(monkeypatch, tmp_path):
