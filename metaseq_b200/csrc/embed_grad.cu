@@ -14,7 +14,7 @@
 //   3. runs that cross borders are joined in ascending order.
 // The launches are chained (programmatic dependent launch), each starts while its predecessor drains.
 // The scatter-add form (embed_ce.cu) needs a zeroed fp32 table, one atomic per element and a pass that folds the table
-// into the 16-bit gradient.  16384 x 2048 bf16 into a new table of 50272 rows: 72 us (0.27 GB: 42 us of copying); 8192 x 768
+// into the 16-bit gradient.  16384 x 2048 bf16 into a new table of 50272 rows: 70 us (0.27 GB: 42 us of copying); 8192 x 768
 // fp16 added to a table: 23 us, of which the sort takes 9.6 and latencies of the two others most of the rest.
 #include "sm100_pair.cuh"
 
@@ -24,7 +24,7 @@ constexpr int EG_CLUSTER = 8;
 constexpr int EG_SORT_THREADS = 1024;
 constexpr int EG_SORT_WARPS = EG_SORT_THREADS / 32;
 constexpr int EG_MAX_BINS = 512;
-constexpr long long EG_FILL_FIRST = 64;  // MB of a new table that are cleared beside the sort (16384 x 2048: 16 MB 81.8 us, 32 MB 80.5, 64 MB 79.0)
+constexpr long long EG_FILL_FIRST = 40;  // MB of a new table that are cleared beside the sort (16384 x 2048: 16 MB 73.1 us, 40 MB 70.0, 64 MB 72.0, 96 MB 76.1)
 
 __device__ __forceinline__ int eg_ld_remote(const int* p, uint32_t rank) {
   int v;
