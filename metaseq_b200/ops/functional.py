@@ -1401,7 +1401,8 @@ def adamw8_step_multi(items, *, lr, beta1, beta2, eps, weight_decay, step, seed,
     probability of the remainder, by a draw from ``seed`` (a non-negative 64-bit number; pass another one every step)
     and the element's number in the list, so equal calls give equal bits.  Values that are not finite (gradients
     beyond 2^52 among them) are stored as NaN.  ``ctrl`` is the device control block of ``clip_decision``: gradients are
-    multiplied by ``ctrl[0]`` and nothing changes when ``ctrl[1] != 0``."""
+    multiplied by ``ctrl[0]`` and nothing changes when ``ctrl[1] != 0``.  All other numbers are read when the call is made: a
+    captured call repeats its step and its draws."""
     items = list(items)
     if not items:
         return
