@@ -28,8 +28,7 @@ F = c_float
 # kernels launched by one call of each entry point (used for the launch counter)
 _KERNELS_PER_CALL = {"msq_flash_head_dim_ok": 0, "msq_symm_alloc": 0, "msq_symm_open": 0, "msq_symm_close": 0, "msq_symm_free": 0, "msq_sumsq": 2, "msq_layernorm_bwd": 2, "msq_rmsnorm_bwd": 2, "msq_flash_bwd": 2, "msq_layernorm_bwd_parts": 0,
                      "msq_sumsq_parts": 0, "msq_gemm2_tiles_n": 0, "msq_gemm_skinny_split": 0, "msq_set_dependent_launch": 0, "msq_gemm_skinny_set_prof": 0, "msq_decode_attn_splits": 0,
-                     "msq_embed_grad_workspace": 0, "msq_embed_grad_sorted": 3,
-                     "msq_lce_saved_bytes": 0, "msq_lce_fwd_bytes": 0, "msq_lce_bwd_bytes": 0, "msq_lce_fwd": 3, "msq_lce_bwd": 4}
+                     "msq_embed_grad_sorted": 3, "msq_lce_fwd": 3, "msq_lce_bwd": 4}
 _LAUNCHES = [0]
 
 
@@ -130,9 +129,6 @@ def _declare_kernels(lib):
     for name, sig in _OPTIONAL.items():
         if hasattr(lib, name):
             _sig(lib, name, sig)
-    for name, sig in _SIZES.items():
-        if hasattr(lib, name):
-            _sig(lib, name, sig, L)
 
 
 # Entry points added by later source files; declared when present.
@@ -210,7 +206,14 @@ def kernels():
             )
         lib = ctypes.CDLL(str(path))
         _declare_kernels(lib)
-        _KLIB = _CountingLib(lib)
+        counting = _CountingLib(lib)
+        # The workspace queries are arithmetic on the host: called without letting go of the interpreter lock (a microsecond
+        # each next to a waiting thread), and not counted.
+        arithmetic = ctypes.PyDLL(str(path))
+        for name, sig in _SIZES.items():
+            if hasattr(lib, name):
+                setattr(counting, name, _sig(arithmetic, name, sig, L))
+        _KLIB = counting
     return _KLIB
 
 

@@ -235,7 +235,7 @@ class LinearCrossEntropyFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index: int):
-        _, total, saved = F.linear_cross_entropy_fwd(x, weight, target, ignore_index)
+        _, total, saved = F._linear_ce_fwd(x, weight, target, ignore_index, False)
         ctx.save_for_backward(weight, target, *saved)
         ctx.param = weight
         ctx.ignore_index = ignore_index
@@ -264,7 +264,7 @@ def linear_cross_entropy_sum(x, weight, target, ignore_index: int):
     exist already."""
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return LinearCrossEntropyFn.apply(x, weight, target, ignore_index)
-    return F.linear_cross_entropy_fwd(x, weight, target, ignore_index)[1]
+    return F._linear_ce_fwd(x, weight, target, ignore_index, False)[1]
 
 
 class EmbeddingFn(torch.autograd.Function):
