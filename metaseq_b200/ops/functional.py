@@ -1431,7 +1431,8 @@ def adamw8_step_multi(items, *, lr, beta1, beta2, eps, weight_decay, step, seed,
     sizes = _adamw8_check(flat)
     if step < 1:
         raise ValueError(f"adamw8_step_multi: the first step is 1, not {step}")
-    addresses = set(map(torch.Tensor.data_ptr, flat[0::6]))
+    pointers = array.array("Q", map(torch.Tensor.data_ptr, flat))
+    addresses = set(pointers[0::6])
     if len(addresses) != len(items) and len(addresses) - (0 in addresses) != len([k for k in sizes if k]):
         raise ValueError("adamw8_step_multi: a parameter stands in the list twice")
     lr, beta1, beta2, eps, weight_decay, seed = float(lr), float(beta1), float(beta2), float(eps), float(weight_decay), int(seed)
@@ -1444,7 +1445,7 @@ def adamw8_step_multi(items, *, lr, beta1, beta2, eps, weight_decay, step, seed,
     step_size = lr * (1.0 - beta2 ** step) ** 0.5 / (1.0 - beta1 ** step)
     decay, omb1, omb2 = lr * weight_decay, 1.0 - beta1, 1.0 - beta2
     if _float_kernels(p0):
-        pointers, counts = array.array("Q", map(torch.Tensor.data_ptr, flat)), array.array("q", sizes)
+        counts = array.array("q", sizes)
         with _on_device(p0):
             rc = _lib.kernels().msq_adamw8_multi(pointers.buffer_info()[0], counts.buffer_info()[0], len(items),
                                                  _lib.dtype_code(p0.dtype), _lib.dtype_code(g0.dtype), beta1, omb1, beta2,
