@@ -999,8 +999,9 @@ def _linear_ce_fwd(x, weight, target, ignore_index: int, rows_too: bool):
     n = tgt.numel()
     ensure_operand_ready(weight)
     if _linear_ce_kernel_ok(x2, weight):
-        if x2.stride(1) != 1 or x2.stride(0) % 8 or x2.data_ptr() % 16:
-            x2 = x2.contiguous()
+        # one row counts as contiguous whatever its row stride, and contiguous() gives back what is contiguous at any address
+        if x2.stride(1) != 1 or x2.data_ptr() % 16 or (n > 1 and x2.stride(0) % 8):
+            x2 = x2.clone(memory_format=torch.contiguous_format)
         lib = _lib.kernels()
         with _on_device(x2):
             kept, scratch = lib.msq_lce_saved_bytes(n, V, D), lib.msq_lce_fwd_bytes(n, V, D)
@@ -1014,7 +1015,7 @@ def _linear_ce_fwd(x, weight, target, ignore_index: int, rows_too: bool):
                 saved = x2.new_empty(kept, dtype=torch.uint8)
                 ws = x2.new_empty(scratch + extra, dtype=torch.uint8)
                 ws_ptr = ws.data_ptr()
-            rc = lib.msq_lce_fwd(x2.data_ptr(), x2.stride(0), weight.data_ptr(), weight.stride(0), tgt.data_ptr(), n, V, D,
+            rc = lib.msq_lce_fwd(x2.data_ptr(), x2.stride(0) if n > 1 else D, weight.data_ptr(), weight.stride(0), tgt.data_ptr(), n, V, D,
                                  int(ignore_index), loss.data_ptr() if rows_too else ws_ptr + scratch, total.data_ptr(),
                                  saved.data_ptr(), ws_ptr, _bf(x2), _lib.status_word(x2.device).data_ptr(), _lib.stream_ptr())
         _lib.check_rc(rc, "msq_lce_fwd")

@@ -296,3 +296,29 @@ def test_graph_replay_with_other_inputs_and_two_streams():
         torch.cuda.synchronize()
         assert all(map(torch.equal, got_a, want_a)) and all(map(torch.equal, got_b, want_b))
     _status_ok("cuda")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n", [1, 60])
+def test_operands_at_odd_addresses(device, n):
+    """Contiguous views at an odd element offset (``contiguous()`` gives them back as they are), and a single row of a wider
+    matrix, which counts as contiguous whatever its row stride."""
+    x, w, t = _inputs(n, 130, 64, torch.bfloat16, device, 21)
+    want = _Oracle(x, w, t)
+
+    def shifted(a, by):
+        return torch.zeros(a.numel() + by, dtype=a.dtype, device=device)[by:].view(a.shape).copy_(a)
+
+    def one_of_many(a):
+        return torch.zeros(3, 67, dtype=a.dtype, device=device)[:1, :64].copy_(a)
+
+    views = [shifted(x, 1), shifted(x, 4)] + ([one_of_many(x)] if n == 1 else [])
+    for a in views:
+        assert a.is_contiguous()
+        for b in (w, shifted(w, 3)):
+            _near(F.linear_cross_entropy(a, b, t, IGN), want.loss, want.loss_off)
+            a, b = a.detach().requires_grad_(), b.detach().requires_grad_()
+            ag.linear_cross_entropy_sum(a, b, t, IGN).backward()
+            _near(a.grad, want.dx, want.dx_off)
+            _near(b.grad, want.dw, want.dw_off)
+    _status_ok(device)
