@@ -1040,7 +1040,8 @@ def linear_cross_entropy_bwd(saved, weight, target, g, ignore_index: int, need_d
                              dw_out: Optional[torch.Tensor] = None, accumulate: bool = False):
     """Gradients ``(dx [*target.shape, D], dw [V, D])`` of ``g * total`` (``g``: one fp32 element on the device).  The
     logits are computed again, a piece of the vocabulary at a time.  ``dw_out`` receives dw (added to what is there with
-    ``accumulate``: one rounding of the sum)."""
+    ``accumulate``: one rounding of the sum).  Where ``dw_out`` is of another type than ``weight``, dw is rounded to the
+    weight's type before."""
     V, D = weight.shape
     tgt = (target if target.dim() == 1 else target.reshape(-1)).contiguous()
     n = tgt.numel()
@@ -1057,21 +1058,22 @@ def linear_cross_entropy_bwd(saved, weight, target, g, ignore_index: int, need_d
         lib = _lib.kernels()
         with _on_device(weight):
             dx = weight.new_empty((*target.shape, D)) if need_dx else None
-            dw = fresh = None
+            dw, same, direct = None, dw_out is not None and dw_out.dtype == weight.dtype, False
             if need_dw:
-                direct = dw_out is not None and dw_out.dtype == weight.dtype and dw_out.stride(1) == 1 \
-                    and dw_out.stride(0) % 8 == 0 and dw_out.stride(0) >= D and dw_out.data_ptr() % 16 == 0
+                direct = same and dw_out.stride(1) == 1 and dw_out.stride(0) % 8 == 0 and dw_out.stride(0) >= D \
+                    and dw_out.data_ptr() % 16 == 0
                 dw = dw_out if direct else weight.new_empty((V, D))
-                fresh = None if direct or dw_out is None else dw
+                if same and accumulate and not direct:  # a layout that the kernel does not take: added to a copy, rounded once as well
+                    dw.copy_(dw_out)
             ws = weight.new_empty(max(16, lib.msq_lce_bwd_bytes(n, V, D, int(need_dx), int(need_dw))), dtype=torch.uint8)
             rc = lib.msq_lce_bwd(weight.data_ptr(), weight.stride(0), tgt.data_ptr(), n, V, D, int(ignore_index),
                                  saved[0].data_ptr(), g.data_ptr(), dx.data_ptr() if need_dx else None, D,
                                  dw.data_ptr() if need_dw else None, dw.stride(0) if need_dw else D,
-                                 int(accumulate and fresh is None), ws.data_ptr(), _bf(weight),
+                                 int(accumulate and same), ws.data_ptr(), _bf(weight),
                                  _lib.status_word(weight.device).data_ptr(), _lib.stream_ptr())
         _lib.check_rc(rc, "msq_lce_bwd")
-        if fresh is not None:  # a table of another type or layout
-            dw_out.copy_(dw_out.float() + fresh.float() if accumulate else fresh)
+        if need_dw and dw_out is not None and not direct:
+            dw_out.copy_(dw_out.float() + dw.float() if accumulate and not same else dw)
             dw = dw_out
         return dx, dw
     x2, lse = saved

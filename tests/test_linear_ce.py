@@ -322,3 +322,20 @@ def test_operands_at_odd_addresses(device, n):
             _near(a.grad, want.dx, want.dx_off)
             _near(b.grad, want.dw, want.dw_off)
     _status_ok(device)
+
+
+@pytest.mark.gpu
+def test_weight_gradient_added_to_an_odd_buffer_is_rounded_once():
+    """A buffer of the weight's type that the kernel cannot write (not 16-byte aligned) gets the bits that an aligned one gets."""
+    x, w, t = _inputs(120, 330, 64, torch.bfloat16, "cuda", 22, 0.1)
+    _, _, saved = F.linear_cross_entropy_fwd(x, w, t, IGN)
+    g = torch.ones((), device="cuda")
+    old = torch.randn(330, 64, device="cuda").bfloat16()
+    for accumulate in (False, True):
+        aligned = old.clone()
+        F.linear_cross_entropy_bwd(saved, w, t, g, IGN, dw_out=aligned, accumulate=accumulate)
+        for odd in (torch.zeros(330 * 64 + 1, dtype=old.dtype, device="cuda")[1:].view(330, 64), torch.zeros(330, 67, dtype=old.dtype, device="cuda")[:, 1:65]):
+            odd.copy_(old)
+            _, dw = F.linear_cross_entropy_bwd(saved, w, t, g, IGN, need_dx=False, dw_out=odd, accumulate=accumulate)
+            assert dw is odd and torch.equal(odd, aligned)
+    _status_ok("cuda")
