@@ -687,11 +687,12 @@ def embed_grad_sorted(tokens, dy, rows: int, scale: float = 1.0, pad_idx: int = 
     _same_device("embed_grad_sorted", tokens, dy, out)
     tok, dy2 = (tokens, dy) if dy.dim() == 2 else (tokens.reshape(-1), dy.reshape(-1, D))
     tok = tok.contiguous()
-    if dy2.stride(1) != 1 or dy2.stride(0) % 8 or dy2.data_ptr() % 16:
-        dy2 = dy2.contiguous()
+    # one row counts as contiguous whatever its row stride, and contiguous() gives back what is contiguous at any address
+    if dy2.stride(1) != 1 or dy2.data_ptr() % 16 or (n > 1 and dy2.stride(0) % 8):
+        dy2 = dy2.clone(memory_format=torch.contiguous_format)
     if _float_kernels(dy2) and D % 8 == 0 and dy2.data_ptr() % 16 == 0 and n <= 1 << 30 and (
-            out is None or (out.dtype == dy2.dtype and out.stride(1) == 1 and out.stride(0) % 8 == 0
-                            and (rows == 1 or out.stride(0) >= D) and out.data_ptr() % 16 == 0
+            out is None or (out.dtype == dy2.dtype and out.stride(1) == 1 and out.data_ptr() % 16 == 0
+                            and (rows == 1 or (out.stride(0) % 8 == 0 and out.stride(0) >= D))
                             and (accumulate or out.is_contiguous()))):
         lib = _lib.kernels()
         with _on_device(dy2):
@@ -699,7 +700,7 @@ def embed_grad_sorted(tokens, dy, rows: int, scale: float = 1.0, pad_idx: int = 
                 out = dy2.new_empty((rows, D))
             size = lib.msq_embed_grad_workspace(n, D)
             ws = dy2.new_empty(size, dtype=torch.uint8) if size else None
-            rc = lib.msq_embed_grad_sorted(tok.data_ptr(), dy2.data_ptr(), dy2.stride(0), out.data_ptr(),
+            rc = lib.msq_embed_grad_sorted(tok.data_ptr(), dy2.data_ptr(), dy2.stride(0) if n > 1 else D, out.data_ptr(),
                                            out.stride(0) if rows > 1 else D, n, rows, D, float(scale), int(vocab_start),
                                            int(pad_idx), int(accumulate), _lib.dtype_code(dy2.dtype),
                                            ws.data_ptr() if size else None, _lib.stream_ptr())

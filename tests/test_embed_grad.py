@@ -186,3 +186,18 @@ def test_large_batches_and_tables(n, rows, D):
     dy = torch.randn(n, D, generator=g, device="cuda").half()
     want, bound = _oracle(tokens, dy, rows, 1.0, -1, 0, None)
     _check(F.embed_grad_sorted(tokens, dy, rows), want, bound)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_one_row_of_a_wider_matrix(device, accumulate):
+    """A single row counts as contiguous whatever its row stride."""
+    dy = torch.randn(3, 67, device=device).half()[:1, :64]
+    old = torch.randn(9, 64, device=device).half() if accumulate else None
+    tokens = torch.tensor([4], device=device)
+    want, bound = _oracle(tokens, dy, 9, 1.5, -1, 0, old)
+    _check(F.embed_grad_sorted(tokens, dy, 9, 1.5, out=old, accumulate=accumulate), want, bound)
+    if accumulate:  # a table of one row
+        out = torch.randn(3, 67, device=device).half()[:1, :64]
+        want, bound = _oracle(tokens - 4, dy, 1, 1.0, -1, 0, out)
+        _check(F.embed_grad_sorted(tokens - 4, dy, 1, out=out, accumulate=True), want, bound)
