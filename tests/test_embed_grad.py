@@ -6,6 +6,7 @@ Bound of an element: the fp32 sum of its k terms and the product with the scale 
 import pytest
 import torch
 
+from metaseq_b200.ops import _lib
 from metaseq_b200.ops import autograd as ag
 from metaseq_b200.ops import functional as F
 
@@ -201,3 +202,42 @@ def test_one_row_of_a_wider_matrix(device, accumulate):
         out = torch.randn(3, 67, device=device).half()[:1, :64]
         want, bound = _oracle(tokens - 4, dy, 1, 1.0, -1, 0, out)
         _check(F.embed_grad_sorted(tokens - 4, dy, 1, out=out, accumulate=True), want, bound)
+
+
+def _captured(call):
+    """A graph of ``call``, which is run once before on another stream."""
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    return graph
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("dtype,other", [(torch.half, torch.float32), (torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16),
+                                         (torch.half, torch.bfloat16)])
+def test_tables_of_another_type_use_the_kernel(dtype, other, accumulate):
+    """Gradients and table of different types: the kernel works in fp32 (its launches are counted, and a captured call repeats)."""
+    g = torch.Generator().manual_seed(8)
+    tokens = torch.randint(0, 60, (700,), generator=g).cuda()
+    dy = torch.randn(700, 40, generator=g).to(dtype).cuda()
+    old = torch.randn(60, 40, generator=g).to(other).cuda()
+    old[7] = -0.0
+    tokens[tokens == 7] = 8
+    want, bound = _oracle(tokens, dy, 60, 1.5, 3, 0, old if accumulate else None)
+    out, before = old.clone(), _lib.launch_count()
+    assert F.embed_grad_sorted(tokens, dy, 60, 1.5, 3, out=out, accumulate=accumulate) is out
+    assert _lib.launch_count() > before
+    _check(out, want, bound + want.abs() * 2.0 ** -24)  # the fp32 result is rounded before the table's type is
+    if accumulate:
+        assert torch.equal(out[7], old[7]) and torch.signbit(out[7]).all() and torch.equal(out[3], old[3])
+    eager = out.clone()
+    graph = _captured(lambda: F.embed_grad_sorted(tokens, dy, 60, 1.5, 3, out=out, accumulate=accumulate))
+    out.copy_(old)
+    graph.replay()
+    assert torch.equal(out, eager)
