@@ -662,6 +662,37 @@ def _same_device(what: str, *tensors):
             raise ValueError(f"{what}: tensors on different devices ({', '.join(devices)})")
 
 
+def _embed_grad_kernel(tok, dy2, rows, scale, pad_idx, vocab_start, out, accumulate):
+    """``embed_grad_sorted`` of flat operands by the kernel.  It takes a ``dy`` and a table of one type, with 16-byte aligned
+    rows whose width is a multiple of eight; anything else goes through a copy of that form (fp32 where the types differ)."""
+    n, D = dy2.shape
+    dtype = dy2.dtype if out is None or out.dtype == dy2.dtype else torch.float32
+    width = -(-D // 8) * 8
+    with _on_device(dy2):
+        if width != D:
+            dy2 = F.pad(dy2, (0, width - D)).to(dtype)
+        # one row counts as contiguous whatever its row stride, and contiguous() gives back what is contiguous at any address
+        elif dy2.dtype != dtype or dy2.stride(1) != 1 or dy2.data_ptr() % 16 or (n > 1 and dy2.stride(0) % 8):
+            dy2 = dy2.to(dtype, copy=True, memory_format=torch.contiguous_format)
+        table = out
+        if out is None or out.dtype != dtype or width != D or out.stride(1) != 1 or out.data_ptr() % 16 or (
+                rows > 1 and (out.stride(0) % 8 or out.stride(0) < D)) or not (accumulate or out.is_contiguous()):
+            table = dy2.new_empty((rows, width))
+            if accumulate:
+                table[:, :D].copy_(out)
+        lib = _lib.kernels()
+        size = lib.msq_embed_grad_workspace(n, width)
+        ws = dy2.new_empty(size, dtype=torch.uint8) if size else None
+        rc = lib.msq_embed_grad_sorted(tok.data_ptr(), dy2.data_ptr(), dy2.stride(0) if n > 1 else width, table.data_ptr(),
+                                       table.stride(0) if rows > 1 else width, n, rows, width, scale, vocab_start, pad_idx,
+                                       int(accumulate), _lib.dtype_code(dtype), ws.data_ptr() if size else None,
+                                       _lib.stream_ptr())
+        _lib.check_rc(rc, "msq_embed_grad_sorted")
+        if out is None:
+            return table if width == D else table[:, :D].contiguous()
+        return out if table is out else out.copy_(table[:, :D])
+
+
 def embed_grad_sorted(tokens, dy, rows: int, scale: float = 1.0, pad_idx: int = -1, vocab_start: int = 0,
                       out: Optional[torch.Tensor] = None, accumulate: bool = False) -> torch.Tensor:
     """Gradient of an embedding lookup written straight into a table of ``dy``'s type:
@@ -670,8 +701,9 @@ def embed_grad_sorted(tokens, dy, rows: int, scale: float = 1.0, pad_idx: int = 
     ``tokens``: int64, any shape; ``dy``: ``[*tokens.shape, D]``; ``rows``: rows of the table (this partition's part of
     the vocabulary).  Tokens equal to ``pad_idx`` or outside the partition contribute nothing; with ``accumulate`` rows
     that no token names are left as they are.  The sums are formed in fp32 over the rows sorted by token, in a fixed
-    order, and rounded once, so equal inputs give equal bits (``embed_bwd`` adds with atomics, in any order).  ``out`` may be
-    of another type than ``dy``: the result is then formed in an fp32 copy of the table."""
+    order, and rounded once, so equal inputs give equal bits (``embed_bwd`` adds with atomics, in any order).  Operands
+    that the kernel does not take as they are (widths that are no multiple of eight, rows that are not 16-byte aligned,
+    ``out`` of another type than ``dy``) are copied for it, the table too."""
     if tokens.dtype != torch.int64:
         raise ValueError(f"embed_grad_sorted: tokens must be int64, not {tokens.dtype}")
     if dy.dim() != tokens.dim() + 1 or dy.shape[:-1] != tokens.shape:
@@ -688,33 +720,10 @@ def embed_grad_sorted(tokens, dy, rows: int, scale: float = 1.0, pad_idx: int = 
     _same_device("embed_grad_sorted", tokens, dy, out)
     tok, dy2 = (tokens, dy) if dy.dim() == 2 else (tokens.reshape(-1), dy.reshape(-1, D))
     tok = tok.contiguous()
-    dtype = dy2.dtype if out is None or out.dtype == dy2.dtype else torch.float32  # what the kernel works in
-    # one row counts as contiguous whatever its row stride, and contiguous() gives back what is contiguous at any address
-    if dy2.stride(1) != 1 or dy2.data_ptr() % 16 or (n > 1 and dy2.stride(0) % 8):
-        dy2 = dy2.clone(memory_format=torch.contiguous_format)
-    table = out
-    if out is not None and out.dtype != dtype:
-        table = out.to(dtype, memory_format=torch.contiguous_format) if accumulate else torch.empty((rows, D), dtype=dtype, device=out.device)
-    if _float_kernels(dy2) and D % 8 == 0 and dy2.data_ptr() % 16 == 0 and n <= 1 << 30 and (
-            table is None or (table.stride(1) == 1 and table.data_ptr() % 16 == 0
-                              and (rows == 1 or (table.stride(0) % 8 == 0 and table.stride(0) >= D))
-                              and (accumulate or table.is_contiguous()))):
-        lib = _lib.kernels()
-        with _on_device(dy2):
-            if dy2.dtype != dtype:
-                dy2 = dy2.to(dtype, memory_format=torch.contiguous_format)
-            if table is None:
-                table = dy2.new_empty((rows, D))
-            size = lib.msq_embed_grad_workspace(n, D)
-            ws = dy2.new_empty(size, dtype=torch.uint8) if size else None
-            rc = lib.msq_embed_grad_sorted(tok.data_ptr(), dy2.data_ptr(), dy2.stride(0) if n > 1 else D, table.data_ptr(),
-                                           table.stride(0) if rows > 1 else D, n, rows, D, float(scale), int(vocab_start),
-                                           int(pad_idx), int(accumulate), _lib.dtype_code(dtype),
-                                           ws.data_ptr() if size else None, _lib.stream_ptr())
-        _lib.check_rc(rc, "msq_embed_grad_sorted")
-        return table if out is None or out is table else out.copy_(table)
+    if _float_kernels(dy2) and n <= 1 << 30:
+        return _embed_grad_kernel(tok, dy2, rows, float(scale), int(pad_idx), int(vocab_start), out, accumulate)
     if dy2.is_cuda and dy2.dtype in (torch.float16, torch.bfloat16):
-        _note_fallback("embed_grad_sorted", f"width {D} must be a multiple of 8, the table's rows 16-byte aligned")
+        _note_fallback("embed_grad_sorted", f"{n} tokens, more than 2^30")
     keep = (tok != pad_idx) & (tok >= vocab_start) & (tok < vocab_start + rows)
     idx = tok[keep] - vocab_start
     table = torch.zeros((rows, D), dtype=torch.float32, device=dy2.device)

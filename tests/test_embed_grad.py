@@ -241,3 +241,54 @@ def test_tables_of_another_type_use_the_kernel(dtype, other, accumulate):
     out.copy_(old)
     graph.replay()
     assert torch.equal(out, eager)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [1, 2, 12, 100, 777])
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("n", [9, 900])
+def test_widths_and_addresses_the_kernel_does_not_take_are_copied(dtype, D, accumulate, n):
+    """Widths that are no multiple of eight, and tables at odd addresses: copied to and from a layout that the kernel takes."""
+    g = torch.Generator().manual_seed(D)
+    tokens = torch.randint(0, 50, (n,), generator=g).cuda()
+    tokens[tokens == 20] = 21
+    dy = torch.randn(n, D, generator=g).to(dtype).cuda()
+    space = torch.randn(50 * D + 3, generator=g).to(dtype).cuda()
+    old = space[1:1 + 50 * D].view(50, D).clone()
+    want, bound = _oracle(tokens, dy, 50, 0.5, 3, 0, old if accumulate else None)
+    before = _lib.launch_count()
+    if not accumulate:
+        got = F.embed_grad_sorted(tokens, dy, 50, 0.5, 3)
+        assert got.shape == (50, D) and got.is_contiguous()
+        _check(got, want, bound)
+    edges = space[[0, -2, -1]].clone()
+    out = space[1:1 + 50 * D].view(50, D)
+    F.embed_grad_sorted(tokens, dy, 50, 0.5, 3, out=out, accumulate=accumulate)
+    assert _lib.launch_count() > before
+    _check(out, want, bound)
+    assert torch.equal(space[[0, -2, -1]], edges)
+    if accumulate:
+        assert torch.equal(out[20], old[20]) and torch.equal(out[3], old[3])
+    wide = torch.full((50, D + 5), 2.0, dtype=dtype, device="cuda")  # rows that lie apart
+    wide[:, :D] = old
+    F.embed_grad_sorted(tokens, dy, 50, 0.5, 3, out=wide[:, :D], accumulate=accumulate)
+    assert torch.equal(wide[:, :D], out) and (wide[:, D:] == 2.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [12, 16])
+def test_embedding_backward_is_captured_at_every_width(D):
+    w = torch.nn.Parameter(torch.randn(60, D, device="cuda").half())
+    w._grad_view, w._grad_filled = torch.zeros(60 * D + 1, dtype=torch.half, device="cuda")[1:].view(60, D), False
+    tokens, up = torch.randint(0, 60, (5, 70), device="cuda"), torch.randn(5, 70, D, device="cuda").half()
+
+    def step():
+        w._grad_filled = False
+        ag.embedding(tokens, None, w, None, 1.0, 3).backward(up)
+
+    graph = _captured(step)
+    tokens.copy_(torch.randint(0, 60, (5, 70), device="cuda"))
+    graph.replay()
+    want, bound = _oracle(tokens, up, 60, 1.0, 3, 0, None)
+    _check(w._grad_view, want, bound)
