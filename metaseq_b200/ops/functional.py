@@ -724,17 +724,17 @@ def embed_grad_sorted(tokens, dy, rows: int, scale: float = 1.0, pad_idx: int = 
         return _embed_grad_kernel(tok, dy2, rows, float(scale), int(pad_idx), int(vocab_start), out, accumulate)
     if dy2.is_cuda and dy2.dtype in (torch.float16, torch.bfloat16):
         _note_fallback("embed_grad_sorted", f"{n} tokens, more than 2^30")
+    # no shape depends on the tokens (a captured call repeats, and nothing waits for the device): one row more takes what
+    # contributes to none
     keep = (tok != pad_idx) & (tok >= vocab_start) & (tok < vocab_start + rows)
-    idx = tok[keep] - vocab_start
-    table = torch.zeros((rows, D), dtype=torch.float32, device=dy2.device)
-    table.index_add_(0, idx, dy2[keep].float() * scale)
+    idx = torch.where(keep, tok - vocab_start, rows)
+    table = torch.zeros((rows + 1, D), dtype=torch.float32, device=dy2.device).index_add_(0, idx, dy2.float() * scale)[:rows]
     if out is None:
         return table.to(dy2.dtype)
-    if not accumulate:
-        return out.copy_(table)
-    hit = torch.unique(idx)
-    out[hit] = (out[hit].float() + table[hit]).to(out.dtype)
-    return out
+    if accumulate:
+        named = torch.zeros(rows + 1, dtype=torch.bool, device=dy2.device).index_fill_(0, idx, True)[:rows, None]
+        table = torch.where(named, (out.float() + table).to(out.dtype), out)
+    return out.copy_(table)
 
 
 def fold_fp32_into(src32: torch.Tensor, dst16: torch.Tensor, accumulate: bool):

@@ -292,3 +292,43 @@ def test_embedding_backward_is_captured_at_every_width(D):
     graph.replay()
     want, bound = _oracle(tokens, up, 60, 1.0, 3, 0, None)
     _check(w._grad_view, want, bound)
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_tensor_form_has_no_shape_that_depends_on_the_tokens(accumulate):
+    """On the meta device there are no values: an operation whose result's shape hangs on them raises."""
+    tokens = torch.zeros(6, 5, dtype=torch.long, device="meta")
+    dy = torch.zeros(6, 5, 12, dtype=torch.half, device="meta")
+    out = torch.zeros(9, 12, dtype=torch.half, device="meta") if accumulate else None
+    assert F.embed_grad_sorted(tokens, dy, 9, out=out, accumulate=accumulate).shape == (9, 12)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_tensor_form_leaves_other_rows_as_they_are(dtype):
+    out = torch.full((4, 3), -0.0, dtype=dtype)
+    out[1] = 1.0 / 3.0
+    old = out.clone()
+    dy = torch.full((3, 3), float("nan"), dtype=dtype)
+    dy[0] = 2.0
+    F.embed_grad_sorted(torch.tensor([2, 7, 3]), dy, 4, pad_idx=3, out=out, accumulate=True)
+    assert torch.equal(out[[0, 1, 3]], old[[0, 1, 3]]) and torch.signbit(out[[0, 3]]).all() and (out[2] == 2.0).all()
+
+
+@pytest.mark.gpu
+def test_tensor_form_is_captured():
+    tokens = torch.randint(0, 60, (300,), device="cuda")
+    dy = torch.randn(300, 12, device="cuda").half()
+    out = torch.ones(60, 12, device="cuda").half()
+
+    def step():
+        F.set_backend("torch")
+        try:
+            F.embed_grad_sorted(tokens, dy, 60, 1.0, 3, out=out, accumulate=True)
+        finally:
+            F.set_backend("auto")
+
+    graph = _captured(step)
+    out.fill_(1.0)
+    graph.replay()
+    want, bound = _oracle(tokens, dy, 60, 1.0, 3, 0, torch.ones(60, 12))
+    _check(out, want, bound)
