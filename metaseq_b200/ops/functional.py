@@ -720,7 +720,8 @@ def embed_grad_sorted(tokens, dy, rows: int, scale: float = 1.0, pad_idx: int = 
     _same_device("embed_grad_sorted", tokens, dy, out)
     tok, dy2 = (tokens, dy) if dy.dim() == 2 else (tokens.reshape(-1), dy.reshape(-1, D))
     tok = tok.contiguous()
-    if _float_kernels(dy2) and n <= 1 << 30:
+    # 32-bit embeddings run without the library as well, like their lookup (use_kernels)
+    if dy2.is_cuda and n <= 1 << 30 and (dy2.dtype != torch.float32 or _lib.kernels_built()) and _float_kernels(dy2):
         return _embed_grad_kernel(tok, dy2, rows, float(scale), int(pad_idx), int(vocab_start), out, accumulate)
     if dy2.is_cuda and dy2.dtype in (torch.float16, torch.bfloat16):
         _note_fallback("embed_grad_sorted", f"{n} tokens, more than 2^30")

@@ -332,3 +332,17 @@ def test_tensor_form_is_captured():
     graph.replay()
     want, bound = _oracle(tokens, dy, 60, 1.0, 3, 0, torch.ones(60, 12))
     _check(out, want, bound)
+
+
+@pytest.mark.gpu
+def test_fp32_embedding_runs_without_the_library(monkeypatch):
+    """Without the built library 32-bit tensors take tensor operations, in both directions; 16-bit ones are refused."""
+    monkeypatch.setattr(_lib, "kernels_built", lambda: False)
+    w = torch.randn(20, 16, device="cuda").requires_grad_()
+    tokens = torch.randint(0, 20, (3, 7), device="cuda")
+    up = torch.randn(3, 7, 16, device="cuda")
+    ag.embedding(tokens, None, w, None, 2.0, 1).backward(up)
+    want, bound = _oracle(tokens, up, 20, 2.0, 1, 0, None)
+    _check(w.grad, want, bound)
+    with pytest.raises(RuntimeError, match="not built"):
+        F.embed_grad_sorted(tokens, up.half(), 20)
