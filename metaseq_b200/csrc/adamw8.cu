@@ -461,13 +461,14 @@ static int launch_adamw8(const unsigned long long* ptrs, const long long* sizes,
   constexpr int smem = a8_smem<PDT, GDT>();
   if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -10;
   kern<<<static_cast<unsigned>(tiles), 256, smem, stream>>>(a);
-  return cudaGetLastError() == cudaSuccess ? 0 : -11;
+  return cudaGetLastError() == cudaSuccess ? 1 : -11;
 }
 
 }  // namespace msq
 
 // Host memory: `ptrs` holds six addresses per tensor, {p, g, codes of m, scales of m, codes of r, scales of r}, `sizes` its
-// elements.  Scales: one fp32 per block of 256 elements.  Tensors with no elements are allowed.
+// elements.  Scales: one fp32 per block of 256 elements.  Tensors with no elements are allowed.  Returns the number of kernels
+// launched, or a negative code.
 extern "C" int msq_adamw8_multi(const unsigned long long* ptrs, const long long* sizes, int count, int p_dtype, int g_dtype, float beta1, float omb1,
                                 float beta2, float omb2, float eps, float decay, float step_size, unsigned long long seed,
                                 const float* ctrl, cudaStream_t stream) {
@@ -475,6 +476,7 @@ extern "C" int msq_adamw8_multi(const unsigned long long* ptrs, const long long*
   constexpr int FEW = 16, MANY = 256;
   const Adam8Hyper h{beta1, omb1, beta2, omb2, eps, decay, step_size, seed, ctrl};
   long long block0 = 0;
+  int launched = 0;
   for (int at = 0; at < count;) {
     const int n = count - at < MANY ? count - at : MANY;
     long long blocks = 0;
@@ -495,9 +497,10 @@ extern "C" int msq_adamw8_multi(const unsigned long long* ptrs, const long long*
     else if (p_dtype == 0 && g_dtype == 2) MSQ_A8(0, 2);
     else if (p_dtype == 1 && g_dtype == 2) MSQ_A8(1, 2);
 #undef MSQ_A8
-    if (rc) return rc;
+    if (rc < 0) return rc;
+    launched += rc;
     block0 += blocks;
     at += n;
   }
-  return 0;
+  return launched;
 }

@@ -707,8 +707,9 @@ extern "C" long long msq_embed_grad_workspace(int n, int D) {
   return ((2LL * n * 8 + 255) & ~255LL) + 2LL * chunks * D * 4;
 }
 
-// See the head of this file.  dtype: 0 fp16, 1 bf16, 2 fp32 (dy and out).  D and both row strides are multiples of eight,
-// dy, out and workspace are 16-byte aligned; a new table (accumulate == 0) has contiguous rows (ldo == D).
+// See the head of this file.  Returns the number of kernels launched, or a negative code.  dtype: 0 fp16, 1 bf16, 2 fp32 (dy
+// and out).  D and both row strides are multiples of eight, dy, out and workspace are 16-byte aligned; a new table
+// (accumulate == 0) has contiguous rows (ldo == D).
 extern "C" int msq_embed_grad_sorted(const long long* tokens, const void* dy, long long ldy, void* out, long long ldo, int n,
                                      int rows, int D, float scale, long long vocab_start, long long pad_idx, int accumulate,
                                      int dtype, void* workspace, cudaStream_t stream) {
@@ -726,11 +727,11 @@ extern "C" int msq_embed_grad_sorted(const long long* tokens, const void* dy, lo
       const long long vecs = rows * vec_per_row, want = (vecs + 2047) / 2048;
       embed_grad_zero_kernel<<<static_cast<unsigned>(want < 4LL * sms ? want : 4LL * sms), 512, 0, stream>>>(static_cast<uint4*>(out), vecs);
       if (cudaGetLastError() != cudaSuccess) return -11;
-      if (n == 0) return 0;
+      if (n == 0) return 1;
     }
     const EmbedGradFew f{tokens, dy, ldy, out, ldo, n, rows, D, accumulate, vocab_start, pad_idx, scale};
     const cudaError_t err = dtype == 0 ? eg_launch_few<0>(f, stream) : dtype == 1 ? eg_launch_few<1>(f, stream) : eg_launch_few<2>(f, stream);
-    return err == cudaSuccess ? 0 : -11;
+    return err == cudaSuccess ? (accumulate ? 1 : 2) : -11;
   }
   EmbedGradSort so;
   so.tokens = tokens;
@@ -782,5 +783,5 @@ extern "C" int msq_embed_grad_sorted(const long long* tokens, const void* dy, lo
   const dim3 join(static_cast<unsigned>((su.chunks + EG_JOIN - 1) / EG_JOIN), static_cast<unsigned>(su.slices));
   const cudaError_t err = dtype == 0 ? eg_launch_sums<0>(su, blocks, join, stream) : dtype == 1 ? eg_launch_sums<1>(su, blocks, join, stream)
                                                                                        : eg_launch_sums<2>(su, blocks, join, stream);
-  return err == cudaSuccess ? 0 : -11;
+  return err == cudaSuccess ? 3 : -11;
 }

@@ -865,7 +865,7 @@ extern "C" long long msq_lce_bwd_bytes(int n, int V, int D, int need_dx, int nee
 
 // loss[n] (0 for ignored rows) and total[0] = their sum; `saved` (msq_lce_saved_bytes) is what the backward pass reads.
 // x [n, D] and w [V, D] are 16-bit, unit inner stride, row strides multiples of eight, 16-byte aligned.  A target that
-// is neither `ignore` nor a column makes the loss of its row NaN.
+// is neither `ignore` nor a column makes the loss of its row NaN.  Returns the number of kernels launched, or a negative code.
 extern "C" int msq_lce_fwd(const void* x, long long ldx, const void* w, long long ldw, const long long* target, int n, int V,
                            int D, long long ignore, float* loss, float* total, void* saved, void* ws, int bf16, int* status,
                            cudaStream_t stream) {
@@ -906,11 +906,12 @@ extern "C" int msq_lce_fwd(const void* x, long long ldx, const void* w, long lon
   LceMerge m;
   m.st_max = st_max; m.st_sum = st_sum; m.st_tgt = st_tgt; m.parts = parts; m.n = n;
   m.rows = sv.rows; m.count = sv.count; m.lse2 = sv.lse2; m.loss = loss; m.partial = partial; m.ticket = ticket; m.total = total;
-  return lce_chain(lce_merge_kernel, (n + 255) / 256 * 8, 1024, 0, stream, true, m);
+  rc = lce_chain(lce_merge_kernel, (n + 255) / 256 * 8, 1024, 0, stream, true, m);
+  return rc ? rc : 3;
 }
 
 // dx [n, D] (0 in ignored rows) and dw [V, D] (added to what is there when `accumulate`), both times g[0]; either may be
-// null.  `saved` from msq_lce_fwd on the same x, w and target.
+// null.  `saved` from msq_lce_fwd on the same x, w and target.  Returns as msq_lce_fwd does.
 extern "C" int msq_lce_bwd(const void* w, long long ldw, const long long* target, int n, int V, int D, long long ignore,
                            const void* saved, const float* g, void* dx, long long lddx, void* dw, long long lddw, int accumulate,
                            void* ws, int bf16, int* status, cudaStream_t stream) {
@@ -936,6 +937,7 @@ extern "C" int msq_lce_bwd(const void* w, long long ldw, const long long* target
   if (rc) return rc;
   rc = make_tmap_2d(&tmXmn, sv.xc, n, D, D, LC_BK, bf16);
   if (rc) return rc;
+  int launched = 0;
   for (int v0 = 0; v0 < V; v0 += q.piece) {
     const int pv = V - v0 < q.piece ? V - v0 : q.piece;
     const uint16_t* wp = static_cast<const uint16_t*>(w) + static_cast<long long>(v0) * ldw;
@@ -948,12 +950,14 @@ extern "C" int msq_lce_bwd(const void* w, long long ldw, const long long* target
     p.M = n; p.N = pv; p.K = D; p.count_is = 1;
     p.target = sv.tgt; p.v0 = v0; p.lse2 = sv.lse2; p.p_log2 = p_log2;
     if ((rc = lce_launch<false, false, LCE_PROB>(tmXk, tmW, tmP, p, sms, stream, v0 > 0))) return rc;
+    ++launched;
     if (dx) {
       if ((rc = make_tmap_2d(&tmPk, P, n, pv, q.piece, LC_BM, bf16))) return rc;
       if ((rc = make_tmap_2d(&tmWmn, wp, pv, D, ldw, LC_BK, bf16))) return rc;
       if ((rc = lce_out_map(&tmOut, dx32, q.dx_rows, D, D, true, bf16))) return rc;
       p.M = n; p.N = D; p.K = pv; p.count_is = 1; p.split_k = q.piece / LC_BK; p.slab_rows = static_cast<int>(q.dx_rows); p.accumulate = v0 > 0;
       if ((rc = lce_launch<false, true, LCE_F32>(tmPk, tmWmn, tmOut, p, sms, stream))) return rc;
+      ++launched;
     }
     if (dw) {
       uint16_t* dwp = static_cast<uint16_t*>(dw) + static_cast<long long>(v0) * lddw;
@@ -963,15 +967,18 @@ extern "C" int msq_lce_bwd(const void* w, long long ldw, const long long* target
         if ((rc = lce_out_map(&tmOut, dw32, q.dw_rows, D, D, true, bf16))) return rc;
         p.accumulate = 0;
         if ((rc = lce_launch<true, true, LCE_F32>(tmPmn, tmXmn, tmOut, p, sms, stream))) return rc;
+        ++launched;
         LceFinish f = {};
         f.acc = dw32; f.pairs = sms / 2; f.slab_rows = p.slab_rows; f.split_count = sv.count; f.D = D; f.M = pv;
         f.out = dwp; f.ldo = lddw; f.g = g; f.alpha = alpha; f.accumulate = accumulate; f.bf16 = bf16;
         const int blocks = (pv + 7) / 8;
         if ((rc = lce_chain(lce_finish_kernel, blocks < 8 * sms ? blocks : 8 * sms, 256, 0, stream, true, f))) return rc;
+        ++launched;
       } else {
         if ((rc = lce_out_map(&tmOut, dwp, pv, D, lddw, false, bf16))) return rc;
         p.accumulate = accumulate; p.out = dwp; p.ldo = lddw; p.g = g;
         if ((rc = lce_launch<true, true, LCE_OUT16>(tmPmn, tmXmn, tmOut, p, sms, stream))) return rc;
+        ++launched;
       }
     }
   }
@@ -982,6 +989,7 @@ extern "C" int msq_lce_bwd(const void* w, long long ldw, const long long* target
     f.out = static_cast<uint16_t*>(dx); f.ldo = lddx; f.g = g; f.alpha = alpha; f.bf16 = bf16;
     const int blocks = (n + 7) / 8;
     if ((rc = lce_chain(lce_finish_kernel, blocks < 8 * sms ? blocks : 8 * sms, 256, 0, stream, true, f))) return rc;
+    ++launched;
   }
-  return 0;
+  return launched;
 }

@@ -25,10 +25,10 @@ L = c_longlong
 F = c_float
 
 
-# kernels launched by one call of each entry point (used for the launch counter)
+# kernels launched by one call of each entry point (used for the launch counter); None: the call returns their number
 _KERNELS_PER_CALL = {"msq_flash_head_dim_ok": 0, "msq_symm_alloc": 0, "msq_symm_open": 0, "msq_symm_close": 0, "msq_symm_free": 0, "msq_sumsq": 2, "msq_layernorm_bwd": 2, "msq_rmsnorm_bwd": 2, "msq_flash_bwd": 2, "msq_layernorm_bwd_parts": 0,
                      "msq_sumsq_parts": 0, "msq_gemm2_tiles_n": 0, "msq_gemm_skinny_split": 0, "msq_set_dependent_launch": 0, "msq_gemm_skinny_set_prof": 0, "msq_decode_attn_splits": 0,
-                     "msq_embed_grad_sorted": 3, "msq_lce_fwd": 3, "msq_lce_bwd": 4}
+                     "msq_embed_grad_sorted": None, "msq_lce_fwd": None, "msq_lce_bwd": None, "msq_adamw8_multi": None}
 _LAUNCHES = [0]
 
 
@@ -54,12 +54,26 @@ class _Counted:
         return self.fn(*args)
 
 
+class _Reporting(_Counted):
+    """The same for an entry point that returns how many kernels it launched, or a negative code."""
+
+    __slots__ = ()
+
+    def __call__(self, *args):
+        rc = self.fn(*args)
+        if rc <= 0:
+            return rc
+        _LAUNCHES[0] += rc
+        return 0
+
+
 class _CountingLib:
     def __init__(self, lib):
         self._lib = lib
 
     def __getattr__(self, name):  # reached once per entry point: the wrapper then is an attribute of its own
-        c = _Counted(getattr(self._lib, name), _KERNELS_PER_CALL.get(name, 1))
+        n = _KERNELS_PER_CALL.get(name, 1)
+        c = (_Reporting if n is None else _Counted)(getattr(self._lib, name), n)
         setattr(self, name, c)
         return c
 

@@ -292,3 +292,50 @@ def test_logits_free_needs_the_whole_vocabulary(monkeypatch, tmp_path):
 
     with pytest.raises(ValueError, match="whole vocabulary"):
         VocabParallelCrossEntropyCriterion(type("T", (), {"target_dictionary": None})(), logits_free=True)
+
+
+def _nodes_of(call):
+    """Launches of a call: the nodes of the graph that it is captured into (the calls below launch nothing but kernels)."""
+    import ctypes
+
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+    count = ctypes.c_size_t(0)
+    get = ctypes.CDLL("libcudart.so.12").cudaGraphGetNodes
+    assert get(ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(count)) == 0
+    return count.value
+
+
+@pytest.mark.gpu
+def test_launch_counter_counts_what_is_launched():
+    w, tokens, target = _step_inputs("cuda", torch.bfloat16)
+    big = torch.randn(20000, 72, device="cuda").bfloat16()
+    few, many = torch.randint(0, 500, (100,), device="cuda"), torch.randint(0, 500, (600,), device="cuda")
+    dy = torch.randn(600, 72, device="cuda").bfloat16()
+    table = torch.zeros(500, 72, device="cuda").bfloat16()
+    x = torch.randn(600, 72, device="cuda").bfloat16()
+    t = torch.randint(0, 20000, (600,), device="cuda")
+    small_t = t % 515
+    one = torch.ones((), device="cuda")
+    _, _, saved = F.linear_cross_entropy_fwd(x, big, t, PAD)
+    _, _, small = F.linear_cross_entropy_fwd(x, w, small_t, PAD)
+    items = [(torch.zeros(300, device="cuda"), torch.zeros(300, device="cuda"), *F.adamw8_state(torch.zeros(300, device="cuda"))) for _ in range(300)]
+    hyper = dict(lr=1e-3, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.0, step=1, seed=1)
+    calls = {
+        "few tokens, new table": lambda: F.embed_grad_sorted(few, dy[:100], 500),
+        "few tokens, added": lambda: F.embed_grad_sorted(few, dy[:100], 500, out=table, accumulate=True),
+        "many tokens": lambda: F.embed_grad_sorted(many, dy, 500),
+        "loss": lambda: F.linear_cross_entropy(x, big, t, PAD),
+        "both gradients": lambda: F.linear_cross_entropy_bwd(saved, big, t, one, PAD),
+        "dx": lambda: F.linear_cross_entropy_bwd(saved, big, t, one, PAD, need_dw=False),
+        "dw": lambda: F.linear_cross_entropy_bwd(small, w, small_t, one, PAD, need_dx=False),
+        "list of 300": lambda: F.adamw8_step_multi(items, **hyper),
+        "list of 5": lambda: F.adamw8_step_multi(items[:5], **hyper),
+    }
+    for name, call in calls.items():
+        call()
+        before = _lib.launch_count()
+        nodes = _nodes_of(call)
+        assert _lib.launch_count() - before == nodes, name
+    assert _lib.check_status("cuda") == 0
