@@ -718,12 +718,12 @@ static int lce_device() {
   cudaGetDevice(&dev);
   return dev;
 }
-static int lce_sms() {
+static int lce_sms() {  // 0 where there is no device to ask
   static std::atomic<int> known[64];
   const int dev = lce_device();
   int sms = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
   if (sms == 0) {
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
     if (dev < 64) known[dev].store(sms, std::memory_order_relaxed);
   }
   return sms;
@@ -855,8 +855,9 @@ extern "C" long long msq_lce_fwd_bytes(int n, int V, int D) {
 // Scratch of the backward pass: one piece of P, the fp32 sums of dx, and those of dw where its rows are split.
 extern "C" long long msq_lce_bwd_bytes(int n, int V, int D, int need_dx, int need_dw) {
   using namespace msq;
-  if (!lce_sizes_ok(n, V, D)) return -1;
-  const LcePlan q = lce_plan(n, V, D, lce_sms());
+  const int sms = lce_sms();
+  if (!lce_sizes_ok(n, V, D) || sms < 2) return -1;
+  const LcePlan q = lce_plan(n, V, D, sms);
   long long b = lce_align(2LL * n * q.piece);
   if (need_dx) b += lce_align(4LL * q.dx_rows * D);
   if (need_dw) b += lce_align(4LL * q.dw_rows * D);
@@ -920,6 +921,7 @@ extern "C" int msq_lce_bwd(const void* w, long long ldw, const long long* target
   if ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(saved) | reinterpret_cast<uintptr_t>(ws) | reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(dw)) & 15) return -4;
   if (!dx && !dw) return 0;
   const int sms = lce_sms();
+  if (sms < 2) return -10;
   const LceSaved sv = lce_saved(const_cast<void*>(saved), n, D);
   const LcePlan q = lce_plan(n, V, D, sms);
   char* at = static_cast<char*>(ws);

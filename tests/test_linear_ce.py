@@ -6,6 +6,10 @@ exponential and logarithm (2^-21 relative to 1 each).  P is off by P * (2 d + 2^
 step, or half the smallest step of fp16 at its factor of 2^15); the gradients are sums of such errors times |w| or |x|,
 the fp32 sums of their terms, and the final rounding.
 """
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -339,3 +343,15 @@ def test_weight_gradient_added_to_an_odd_buffer_is_rounded_once():
             _, dw = F.linear_cross_entropy_bwd(saved, w, t, g, IGN, need_dx=False, dw_out=odd, accumulate=accumulate)
             assert dw is odd and torch.equal(odd, aligned)
     _status_ok("cuda")
+
+
+def test_workspace_queries_answer_without_a_device():
+    """The size of the scratch depends on the device: without one the query says so and does not end the process."""
+    if not _lib.kernels_built():
+        pytest.skip("library not built")
+    code = ("from metaseq_b200.ops import _lib; lib = _lib.kernels(); "
+            "print(lib.msq_lce_saved_bytes(100, 200, 64), lib.msq_lce_fwd_bytes(100, 200, 64), lib.msq_lce_bwd_bytes(100, 200, 64, 1, 1))")
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, env={**os.environ, "CUDA_VISIBLE_DEVICES": ""})
+    assert run.returncode == 0, run.stderr
+    saved, fwd, bwd = map(int, run.stdout.split())
+    assert saved > 2 * 100 * 64 and fwd > 0 and bwd == -1
