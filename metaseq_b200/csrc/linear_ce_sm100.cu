@@ -888,10 +888,12 @@ extern "C" int msq_lce_fwd(const void* x, long long ldx, const void* w, long lon
   c.x = static_cast<const uint4*>(x); c.ldx = ldx / 8; c.xc = reinterpret_cast<uint4*>(sv.xc); c.vecs = D / 8;
   c.target = target; c.ignore = ignore; c.n = n; c.V = V; c.rows = sv.rows; c.tgt = sv.tgt; c.st_tgt = st_tgt;
   c.count = sv.count; c.ticket = ticket; c.loss = loss;
-  lce_compact_kernel<<<(n + LC_COMPACT_ROWS - 1) / LC_COMPACT_ROWS, 256, 0, stream>>>(c);
+  // (the kernels behind it take their sizes from what it leaves)
+  int rc = lce_chain(lce_compact_kernel, (n + LC_COMPACT_ROWS - 1) / LC_COMPACT_ROWS, 256, 0, stream, false, c);
+  if (rc) return rc;
 
   CUtensorMap tmA, tmB;
-  int rc = make_tmap_2d(&tmA, sv.xc, n, D, D, LC_BM, bf16);
+  rc = make_tmap_2d(&tmA, sv.xc, n, D, D, LC_BM, bf16);
   if (rc) return rc;
   rc = make_tmap_2d(&tmB, w, V, D, ldw, LC_BN / 2, bf16);
   if (rc) return rc;

@@ -355,3 +355,15 @@ def test_workspace_queries_answer_without_a_device():
     assert run.returncode == 0, run.stderr
     saved, fwd, bwd = map(int, run.stdout.split())
     assert saved > 2 * 100 * 64 and fwd > 0 and bwd == -1
+
+
+def test_failed_launches_are_reported():
+    """Without a device no kernel starts: the first launch of a call says so (what follows reads what it leaves)."""
+    if not _lib.kernels_built():
+        pytest.skip("library not built")
+    code = ("import torch; from metaseq_b200.ops import _lib; lib = _lib.kernels(); b = torch.zeros(1 << 16); p = b.data_ptr() + 63 & ~63; "
+            "print(lib.msq_lce_fwd(p, 64, p, 64, p, 4, 8, 64, 1, p, p, p, p, 1, None, None), "
+            "lib.msq_lce_bwd(p, 64, p, 4, 8, 64, 1, p, p, p, 64, p, 64, 0, p, 1, None, None))")
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, env={**os.environ, "CUDA_VISIBLE_DEVICES": ""})
+    assert run.returncode == 0, run.stderr
+    assert run.stdout.split() == ["-11", "-10"]
