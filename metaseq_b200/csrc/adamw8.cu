@@ -474,6 +474,8 @@ extern "C" int msq_adamw8_multi(const unsigned long long* ptrs, const long long*
                                 const float* ctrl, cudaStream_t stream) {
   using namespace msq;
   constexpr int FEW = 16, MANY = 256;
+  const int sms = device_sms();
+  if (sms <= 0) return -10;
   const Adam8Hyper h{beta1, omb1, beta2, omb2, eps, decay, step_size, seed, ctrl};
   long long block0 = 0;
   int launched = 0;
@@ -483,7 +485,7 @@ extern "C" int msq_adamw8_multi(const unsigned long long* ptrs, const long long*
     for (int i = 0; i < n; ++i) blocks += (sizes[at + i] + A8_BLOCK - 1) / A8_BLOCK;
     // A CTA's tile: long ones save the start-up of the copies (403M elements: 32 blocks 866 us, 128 blocks 831 us), but six
     // tiles an SM keep the last wave short (6.3M fp32 elements: 8 blocks 26.4 us, 24 blocks 20.8 us, 56 blocks 22.6 us).
-    long long tile = blocks / (6 * 148) / 8 * 8;
+    const long long tile = blocks / (6 * sms) / 8 * 8;
     const int tile_blocks = static_cast<int>(tile < 8 ? 8 : tile > 128 ? 128 : tile);
     int rc = -2;
 #define MSQ_A8(PD, GD)                                                                                      \

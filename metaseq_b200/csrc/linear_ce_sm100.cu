@@ -713,28 +713,13 @@ static int lce_chain(void (*kernel)(KArgs...), unsigned grid, unsigned block, si
   return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? 0 : -11;
 }
 
-static int lce_device() {
-  int dev = 0;
-  cudaGetDevice(&dev);
-  return dev;
-}
-static int lce_sms() {  // 0 where there is no device to ask
-  static std::atomic<int> known[64];
-  const int dev = lce_device();
-  int sms = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
-  if (sms == 0) {
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-    if (dev < 64) known[dev].store(sms, std::memory_order_relaxed);
-  }
-  return sms;
-}
-
 template <bool A_MN, bool B_MN, int EPI>
 static int lce_launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmC, const LceParams& p, int sms,
                       cudaStream_t stream, bool chained = true) {
   auto kern = lce_gemm_kernel<A_MN, B_MN, EPI>;
   static std::atomic<unsigned long long> configured{0};  // a bit per device
-  const int dev = lce_device();
+  int dev = 0;
+  cudaGetDevice(&dev);
   const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
   if (!(configured.load(std::memory_order_relaxed) & bit)) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, LC_SMEM) != cudaSuccess) return -10;
@@ -855,7 +840,7 @@ extern "C" long long msq_lce_fwd_bytes(int n, int V, int D) {
 // Scratch of the backward pass: one piece of P, the fp32 sums of dx, and those of dw where its rows are split.
 extern "C" long long msq_lce_bwd_bytes(int n, int V, int D, int need_dx, int need_dw) {
   using namespace msq;
-  const int sms = lce_sms();
+  const int sms = device_sms();
   if (!lce_sizes_ok(n, V, D) || sms < 2) return -1;
   const LcePlan q = lce_plan(n, V, D, sms);
   long long b = lce_align(2LL * n * q.piece);
@@ -903,7 +888,7 @@ extern "C" int msq_lce_fwd(const void* x, long long ldx, const void* w, long lon
   p.bf16 = bf16; p.status = status;
   p.target = sv.tgt;
   p.st_max = st_max; p.st_sum = st_sum; p.st_tgt = st_tgt;
-  rc = lce_launch<false, false, LCE_STATS>(tmA, tmB, tmA, p, lce_sms(), stream);
+  rc = lce_launch<false, false, LCE_STATS>(tmA, tmB, tmA, p, device_sms(), stream);
   if (rc) return rc;
 
   LceMerge m;
@@ -922,7 +907,7 @@ extern "C" int msq_lce_bwd(const void* w, long long ldw, const long long* target
   if (!lce_sizes_ok(n, V, D) || (ldw & 7) || (lddx & 7) || (lddw & 7)) return -4;
   if ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(saved) | reinterpret_cast<uintptr_t>(ws) | reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(dw)) & 15) return -4;
   if (!dx && !dw) return 0;
-  const int sms = lce_sms();
+  const int sms = device_sms();
   if (sms < 2) return -10;
   const LceSaved sv = lce_saved(const_cast<void*>(saved), n, D);
   const LcePlan q = lce_plan(n, V, D, sms);

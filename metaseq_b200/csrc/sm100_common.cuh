@@ -12,7 +12,22 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace msq {
+
+// SMs of the current device, asked once per device; 0 where there is none to ask.
+inline int device_sms() {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int sms = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (sms == 0) {
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    if (dev < 64) known[dev].store(sms, std::memory_order_relaxed);
+  }
+  return sms;
+}
 
 // Status codes written to the int status word of a launch (0 = ok).
 enum : int {
