@@ -206,3 +206,75 @@ def test_refusals():
     with pytest.raises(ValueError, match="control block"):
         step(*ok, ctrl=torch.zeros(4, dtype=torch.float64))
     F.adamw8_step_multi([], **HYPER, step=1, seed=0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pdt,gdt", PAIRS)
+def test_long_lists_turn_the_ring(pdt, gdt):
+    """Lists whose warps take more blocks one after the other than the ring of copies has stages (46,000 blocks: six a warp
+    and more), with odd tails: scales and codes equal the restatement's bit by bit."""
+    sizes = [11_900_123, 7, 70_001]
+    g = torch.Generator(device="cuda").manual_seed(6)
+    here = []
+    for n in sizes:
+        blocks = -(-n // 256)
+        p = torch.randn(n, generator=g, device="cuda").to(pdt)
+        grad = (torch.randn(n, generator=g, device="cuda") * 10 ** (4 * torch.rand(n, generator=g, device="cuda") - 5)).to(gdt)
+        m = (torch.randn(n, generator=g, device="cuda") * 100).clamp(-448, 448).to(torch.float8_e4m3fn)
+        r = (torch.randn(n, generator=g, device="cuda").abs() * 100).clamp(2.0 ** -9, 448).to(torch.float8_e4m3fn)
+        scales = [torch.exp2(torch.randint(-20, -10, (blocks,), generator=g, device="cuda").float()) for _ in range(2)]
+        here.append((p, grad, m, scales[0], r, scales[1]))
+    there = [tuple(t.clone() for t in item) for item in here]
+    F.adamw8_step_multi(here, **HYPER, step=3, seed=77)
+    F.set_backend("torch")
+    try:
+        F.adamw8_step_multi(there, **HYPER, step=3, seed=77)
+    finally:
+        F.set_backend("auto")
+    _same_update(here, there, pdt)
+
+
+def _same_update(here, there, pdt):
+    """The parameters differ by the kernel's quotient (2^-22 of the step) and by five roundings of 2^-24 of the old value, the
+    step and the new value; the step is at most the new value and the old one, which is below 6: 2^-20 of both together, and
+    a whole step of p's type where the two lie on either side of a border."""
+    for a, b in zip(here, there):
+        for k in (2, 3, 4, 5):
+            assert torch.equal(a[k].view(torch.uint8), b[k].view(torch.uint8))
+        p, q = a[0].double(), b[0].double()
+        assert ((p == q) | ((p - q).abs() <= (q.abs() + 8.0) * 2.0 ** -20 + torch.finfo(pdt).eps * q.abs())).all()
+
+
+@pytest.mark.gpu
+def test_element_numbers_beyond_32_bits(monkeypatch):
+    """The draws of a list that passes 2^32 elements inside a tensor, in the middle of a warp's run of blocks: windows around the
+    border, at the start and at the end equal the restatement, which is given the windows' first element numbers."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 26 GB")
+    lead, n = 5 * 256, (1 << 32) + 300_000
+    zeros = lambda k, dt: torch.zeros(k, dtype=torch.uint8, device="cuda").view(dt)  # noqa: E731
+    p, g, m, r = zeros(2 * n, torch.bfloat16), zeros(2 * n, torch.bfloat16), zeros(n, torch.float8_e4m3fn), zeros(n, torch.float8_e4m3fn)
+    ms, rs = torch.ones(-(-n // 256), device="cuda"), torch.ones(-(-n // 256), device="cuda")
+    border = ((1 << 32) - lead) // 256  # block of the tensor at which the element number passes 2^32
+    windows = [(0, 40), (border - 700, border + 700), (len(ms) - 300, len(ms))]
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    for b0, b1 in windows:
+        a, b = b0 * 256, min(b1 * 256, n)
+        p[a:b] = torch.randn(b - a, generator=gen, device="cuda").bfloat16()
+        g[a:b] = (torch.randn(b - a, generator=gen, device="cuda") * 1e-3).bfloat16()
+        m[a:b] = (torch.randn(b - a, generator=gen, device="cuda") * 100).clamp(-448, 448).to(torch.float8_e4m3fn)
+        r[a:b] = (torch.randn(b - a, generator=gen, device="cuda").abs() * 100).clamp(2.0 ** -9, 448).to(torch.float8_e4m3fn)
+        ms[b0:b1], rs[b0:b1] = 2.0 ** -14, 2.0 ** -15
+    cut = lambda b0, b1: tuple(t[b0 * 256:min(b1 * 256, n)] for t in (p, g, m)) + (ms[b0:b1], r[b0 * 256:min(b1 * 256, n)], rs[b0:b1])  # noqa: E731
+    wants = [tuple(t.clone() for t in cut(b0, b1)) for b0, b1 in windows]
+    first = torch.zeros(lead, dtype=torch.bfloat16, device="cuda")
+    F.adamw8_step_multi([(first, torch.zeros_like(first), *F.adamw8_state(first)), (p, g, m, ms, r, rs)], **HYPER, step=2, seed=(9 << 33) + 1)
+    draws = F._adamw8_draws
+    F.set_backend("torch")
+    try:
+        for (b0, b1), want in zip(windows, wants):
+            monkeypatch.setattr(F, "_adamw8_draws", lambda blocks, at, seed, device: draws(blocks, at + 5 + b0, seed, device))
+            F.adamw8_step_multi([want], **HYPER, step=2, seed=(9 << 33) + 1)
+    finally:
+        F.set_backend("auto")
+    _same_update([cut(b0, b1) for b0, b1 in windows], wants, torch.bfloat16)
