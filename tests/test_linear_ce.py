@@ -367,3 +367,39 @@ def test_failed_launches_are_reported():
     run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, env={**os.environ, "CUDA_VISIBLE_DEVICES": ""})
     assert run.returncode == 0, run.stderr
     assert run.stdout.split() == ["-11", "-10"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,V,D", [(513, 300, 328), (700, 129, 72), (1500, 600, 64)])
+def test_weight_gradient_in_parts_is_added_to_a_buffer(dtype, n, V, D):
+    """Sizes whose rows are cut into parts: fp32 slabs, joined into the buffer when it is filled and when it is added to."""
+    lib = _lib.kernels()
+    assert lib.msq_lce_bwd_bytes(n, V, D, 0, 1) > lib.msq_lce_bwd_bytes(n, V, D, 0, 0)  # the slabs
+    x, w, t = _inputs(n, V, D, dtype, "cuda", 23, 0.1)
+    want = _Oracle(x, w, t)
+    w = torch.nn.Parameter(w)
+    half = torch.finfo(dtype).eps / 2
+    wide = torch.full((V, D + 16), 3.0, dtype=dtype, device="cuda")  # rows that lie apart
+    for view in (torch.full((V, D), float("nan"), dtype=dtype, device="cuda"), wide[:, 8:8 + D]):
+        w._grad_view, w._grad_filled = view, False
+        for k in (1, 2, 3):  # micro-batches: every sum is rounded to the buffer's type
+            ag.linear_cross_entropy_sum(x, w, t, IGN).backward()
+            assert w.grad is None
+            _near(view, k * want.dw, k * (1 + 4 * half) * want.dw_off + half * want.dw.abs() * sum(range(1, k)))
+    assert (wide[:, :8] == 3.0).all() and (wide[:, 8 + D:] == 3.0).all()
+    _status_ok("cuda")
+
+
+@pytest.mark.gpu
+def test_equal_inputs_give_equal_bits():
+    """Pieces and parts are added in a fixed order."""
+    for n, V, D in ((513, 300, 328), (2000, 30011, 136), (37, 1021, 64)):
+        x, w, t = _inputs(n, V, D, torch.bfloat16, "cuda", 24, 0.2)
+        results = []
+        for _ in range(4):
+            loss, total, saved = F.linear_cross_entropy_fwd(x, w, t, IGN)
+            results.append((loss, total, *F.linear_cross_entropy_bwd(saved, w, t, torch.ones((), device="cuda"), IGN)))
+        for other in results[1:]:
+            assert all(map(torch.equal, other, results[0]))
+    _status_ok("cuda")
