@@ -346,3 +346,24 @@ def test_fp32_embedding_runs_without_the_library(monkeypatch):
     _check(w.grad, want, bound)
     with pytest.raises(RuntimeError, match="not built"):
         F.embed_grad_sorted(tokens, up.half(), 20)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,n,rows,D", [(torch.float32, 3000, 30011, 1000), (torch.float32, 700, 20011, 1032), (torch.bfloat16, 5000, 50272, 776),
+                                            (torch.float16, 300, 41003, 1544), (torch.bfloat16, 70001, 60007, 520)])
+@pytest.mark.parametrize("kind", ["uniform", "frequent"])
+def test_new_tables_larger_than_what_is_cleared_beside_the_sort(dtype, n, rows, D, kind):
+    """Tables over 40 MB of wide rows: the rows behind that are cleared unless a token names them."""
+    assert rows * D * dtype.itemsize > 40 << 20
+    tokens = _tokens(kind, n, rows, 0, torch.Generator().manual_seed(n))
+    tokens[:3] = torch.tensor([0, rows - 1, rows - 2])
+    tokens = tokens.cuda()
+    dy = torch.randn(n, D, generator=torch.Generator(device="cuda").manual_seed(n), device="cuda").to(dtype)
+    out = torch.full((rows, D), float("nan"), dtype=dtype, device="cuda")
+    F.embed_grad_sorted(tokens, dy, rows, 1.5, 1, out=out)
+    keep = tokens != 1
+    named, place = torch.unique(tokens[keep], return_inverse=True)
+    want, bound = _oracle(place, dy[keep], len(named), 1.5, -1, 0, None)
+    _check(out[named], want, bound)
+    out[named] = 0
+    assert (out == 0).all()
