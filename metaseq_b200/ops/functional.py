@@ -618,7 +618,7 @@ def embed_bwd(tokens, positions, dy, tok_rows: int, pos_rows: int, scale: float,
     vocab_end = vocab_start + tok_rows
     dtok = torch.zeros((tok_rows, D), dtype=torch.float32, device=dy.device)
     dpos = torch.zeros((pos_rows, D), dtype=torch.float32, device=dy.device) if flat_pos is not None else None
-    if use_kernels(dy2) and D % 2 == 0 and dy2.is_contiguous():
+    if use_kernels(dy2) and D % 2 == 0 and dy2.is_contiguous() and dy2.data_ptr() % 4 == 0:  # it reads pairs
         rc = _lib.kernels().msq_embed_bwd(
             _lib.ptr(flat_tok), _lib.ptr(flat_pos), _lib.ptr(dy2), _lib.ptr(dtok), _lib.ptr(dpos),
             dy2.shape[0], D, float(scale), int(vocab_start), int(vocab_end), int(pad_idx), _bf(dy2),
@@ -741,7 +741,7 @@ def embed_grad_sorted(tokens, dy, rows: int, scale: float = 1.0, pad_idx: int = 
 def fold_fp32_into(src32: torch.Tensor, dst16: torch.Tensor, accumulate: bool):
     """``dst16 (+)= src32`` elementwise, with the sum formed in fp32."""
     n = src32.numel()
-    if use_kernels(dst16) and n % 2 == 0 and dst16.is_contiguous() and src32.is_contiguous():
+    if use_kernels(dst16) and n % 2 == 0 and dst16.is_contiguous() and src32.is_contiguous() and dst16.data_ptr() % 4 == 0:  # it writes pairs
         rc = _lib.kernels().msq_fold_fp32(_lib.ptr(src32), _lib.ptr(dst16), n, int(accumulate), _bf(dst16),
                                           _lib.stream_ptr())
         _lib.check_rc(rc, "msq_fold_fp32")

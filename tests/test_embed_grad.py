@@ -367,3 +367,20 @@ def test_new_tables_larger_than_what_is_cleared_beside_the_sort(dtype, n, rows, 
     _check(out[named], want, bound)
     out[named] = 0
     assert (out == 0).all()
+
+
+@pytest.mark.gpu
+def test_pairs_at_odd_addresses():
+    """16-bit tensors at an odd element offset: the kernels that read or write two values at once are not given them."""
+    g = torch.Generator().manual_seed(1)
+    tokens = torch.randint(0, 40, (300,), generator=g).cuda()
+    space = torch.randn(300 * 12 + 1, generator=g).half().cuda()
+    dy = space[1:].view(300, 12)
+    assert dy.is_contiguous() and dy.data_ptr() % 4 == 2
+    want, bound = _oracle(tokens, dy, 40, 1.5, 3, 0, None)
+    table, _ = F.embed_bwd(tokens, None, dy, 40, 0, 1.5, 3, need_pos=False)
+    _check(table, want, bound)
+    for accumulate in (False, True):
+        room = torch.ones(40 * 12 + 2, dtype=torch.half, device="cuda")
+        F.fold_fp32_into(table, room[1:-1].view(40, 12), accumulate)
+        assert torch.equal(room[1:-1].view(40, 12), (table + float(accumulate)).half()) and room[0] == 1 and room[-1] == 1
