@@ -384,3 +384,34 @@ def test_pairs_at_odd_addresses():
         room = torch.ones(40 * 12 + 2, dtype=torch.half, device="cuda")
         F.fold_fp32_into(table, room[1:-1].view(40, 12), accumulate)
         assert torch.equal(room[1:-1].view(40, 12), (table + float(accumulate)).half()) and room[0] == 1 and room[-1] == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [12, 100, 18])
+@pytest.mark.parametrize("views", [False, True])
+def test_embedding_backward_of_even_widths_scatters(monkeypatch, dtype, D, views):
+    """16-bit rows of an even width that is no multiple of eight: the kernel that scatters with atomics, for both tables."""
+    calls, scatter = [], F.embed_bwd
+    monkeypatch.setattr(F, "embed_bwd", lambda *a, **k: calls.append(1) or scatter(*a, **k))
+    g = torch.Generator().manual_seed(D)
+    tok_w, pos_w = (torch.nn.Parameter(torch.randn(k, D, generator=g).to(dtype).cuda()) for k in (50, 30))
+    tokens = torch.randint(0, 50, (4, 25), generator=g).cuda()
+    tokens[2, 9:] = 1
+    positions = torch.where(tokens == 1, 1, torch.arange(25, device="cuda") + 2)
+    up = torch.randn(4, 25, D, generator=g).to(dtype).cuda()
+    if views:
+        for w in (tok_w, pos_w):
+            w._grad_view, w._grad_filled = torch.full(w.shape, float("nan"), dtype=dtype, device="cuda"), False
+    before = _lib.launch_count()
+    ag.embedding(tokens, positions, tok_w, pos_w, 2.0, 1).backward(up)
+    assert calls == [1] and _lib.launch_count() > before
+    for w, index, scale in ((tok_w, tokens, 2.0), (pos_w, positions, 1.0)):
+        want, bound = _oracle(index, up, len(w), scale, 1, 0, None)
+        _check(w._grad_view if views else w.grad, want, bound)
+        assert not views or w.grad is None
+    if not views:
+        tok_w.grad = None
+        ag.embedding(tokens, positions[:1], tok_w, None, 2.0, 1).backward(up)  # no position table: the numbers are not looked at
+        want, bound = _oracle(tokens, up, 50, 2.0, 1, 0, None)
+        _check(tok_w.grad, want, bound)
