@@ -356,16 +356,6 @@ adamw_multi_kernel(const AdamTensor* __restrict__ table, float lr, float beta1, 
   }
 }
 
-static int device_sms() {
-  static int sms = 0;
-  if (!sms) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  }
-  return sms;
-}
-
 }  // namespace msq
 
 // Number of scratch floats msq_sumsq needs for an n-element tensor.
