@@ -24,7 +24,10 @@ constexpr int EG_CLUSTER = 8;
 constexpr int EG_SORT_THREADS = 1024;
 constexpr int EG_SORT_WARPS = EG_SORT_THREADS / 32;
 constexpr int EG_MAX_BINS = 512;
-constexpr long long EG_FILL_FIRST = 40;  // MB of a new table that are cleared beside the sort (16384 x 2048: 16 MB 73.1 us, 40 MB 70.0, 64 MB 72.0, 96 MB 76.1)
+// MB of a new table that are cleared beside the sort: what the sort of up to 16384 tokens covers.  16, 40, 64 and 128 MB of a
+// bf16 table of 50272 x 2048, us in a graph: 300 tokens 43.9, 42.8, 47.9, 53.6; 8192 55.5, 55.2, 60.1, 66.3; 16384 70.8, 66.7,
+// 69.7, 76.3.  The longer radix sort of more tokens would cover more: 32768 109.5, 106.8, 106.2, 96.8; 131072 263, 263, 263, 258.
+constexpr long long EG_FILL_FIRST = 40;
 
 __device__ __forceinline__ int eg_ld_remote(const int* p, uint32_t rank) {
   int v;
@@ -573,7 +576,11 @@ __global__ void __launch_bounds__(256) embed_grad_join_kernel(const EmbedGradSum
 
 // Few tokens: a CTA per 256 columns finds every token's place by counting (equal tokens keep their order), its 16 warps sum
 // contiguous parts of the sorted list, and runs that cross from one warp to the next are joined through shared memory.
-constexpr int EG_FEW = 256;  // tokens.  768 columns: 128 tokens 5.8 us (three launches 14.1), 256 11.1 (14.5), 400 20.1 (14.8)
+// Tokens up to which this is taken: one kernel against three launches, us in a graph.  Added, 768 columns in 16 bits: 128 tokens 6.3
+// (14.3), 256 11.1 (14.5), 320 14.9 (14.7), 400 20.8 (14.9); 256 tokens of 64 columns 11.3 (14.9), of 4096 11.6 (15.0), of 768 in
+// fp32 13.0 (14.8).  Wide new tables are behind, since nothing hides their clearing: 2050 rows of 4096, 192 tokens 15.0 (14.5), 256
+// 18.0 (14.8).
+constexpr int EG_FEW = 256;
 constexpr int EG_FEW_THREADS = 512;
 constexpr int EG_FEW_WARPS = EG_FEW_THREADS / 32;
 

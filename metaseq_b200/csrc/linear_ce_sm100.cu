@@ -18,8 +18,8 @@
 //
 // What bounds it is the tensor pipe: active 88 to 93 % of the cycles in all four products (8192 x 9472 x 2048 bf16, 1.5 to
 // 1.6 PFLOP/s), with the clock lowered by the power limit in long runs.  16384 rows, 50272 columns, width 2048, fp16, loss
-// and both gradients: 10.7 to 11.1 ms (13.5 TFLOP with the logits computed twice), scratch 0.4 GB where the logits alone
-// would take 1.6.  Smaller 16-bit output tiles from two staging buffers a warp (64-byte rows) changed nothing.  Few tiles (short
+// and both gradients: 10.7 to 11.4 ms with 3.7 % of the rows ignored (13.0 TFLOP with the logits computed twice), 11.1 to 11.7 with
+// all rows kept (13.5 TFLOP), scratch 0.4 GB where the logits alone would take 1.6.  Smaller 16-bit output tiles from two staging buffers a warp (64-byte rows) changed nothing.  Few tiles (short
 // pieces, few kept rows) are cut along K into fp32 slabs that are added in order (lce_splits): no atomics, equal inputs give
 // equal bits.
 #include <atomic>
@@ -456,7 +456,9 @@ lce_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 }
 
 // Kept rows to the front of `xc`, in order: a CTA counts the kept rows before its 32 and copies its own.  The last CTA
-// leaves the count and clears the rows up to the next multiple of 256 (the products read whole tiles).
+// leaves the count and clears the rows up to the next multiple of 256 (the products read whole tiles).  The counting reads
+// n^2 / 8 bytes of targets, from L2: 34 MB at 16384 rows; 137 GB at a million, about half of the 6.3 ms that their loss takes over
+// 1024 columns of width 64 (131072 rows: 0.35 ms).
 constexpr int LC_COMPACT_ROWS = 32;
 
 struct LceCompact {
@@ -754,8 +756,9 @@ struct LcePlan {
 };
 
 // The size of a piece is the one whose three products have the shortest waves (units as in lce_splits, ten for a launch),
-// P staying within 256 MB; ignored rows are not known here.  16384 rows, 50272 columns, width 2048: pieces of 4096 columns
-// (dw: 128 tiles for 74 pairs) 11.34 ms, of 4608 (144 tiles) 11.11 ms.
+// P staying within 256 MB (above 131072 rows within 2 KB a row: four tiles); ignored rows are not known here.  16384 rows, 50272
+// columns, width 2048, all kept, one run after the other: pieces of 4096 columns (dw: 128 tiles for 74 pairs) 11.8 ms, of 4608
+// (144 tiles) 11.6, of 6912 (216 tiles; the choice) 11.5, of 8192 11.9.
 static LcePlan lce_plan(int n, int V, int D, int sms) {
   LcePlan q;
   const int pairs = sms / 2;
