@@ -18,10 +18,10 @@
 //
 // What bounds it is the tensor pipe: active 88 to 93 % of the cycles in all four products (8192 x 9472 x 2048 bf16, 1.5 to
 // 1.6 PFLOP/s), with the clock lowered by the power limit in long runs.  16384 rows, 50272 columns, width 2048, fp16, loss
-// and both gradients: 10.7 to 11.4 ms with 3.7 % of the rows ignored (13.0 TFLOP with the logits computed twice), 11.1 to 11.7 with
-// all rows kept (13.5 TFLOP), scratch 0.4 GB where the logits alone would take 1.6.  Smaller 16-bit output tiles from two staging buffers a warp (64-byte rows) changed nothing.  Few tiles (short
-// pieces, few kept rows) are cut along K into fp32 slabs that are added in order (lce_splits): no atomics, equal inputs give
-// equal bits.
+// and both gradients: 10.7 to 11.4 ms with 3.7 % of the rows ignored (13.0 TFLOP with the logits computed twice), 11.1 to
+// 11.7 ms with all rows kept (13.5 TFLOP); scratch 0.4 GB where the logits alone would take 1.6.  Smaller 16-bit output tiles
+// from two staging buffers a warp (64-byte rows) changed nothing.  Few tiles (short pieces, few kept rows) are cut along K
+// into fp32 slabs that are added in order (lce_splits): no atomics, equal inputs give equal bits.
 #include <atomic>
 
 #include "sm100_pair.cuh"
